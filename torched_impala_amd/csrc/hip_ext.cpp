@@ -13,6 +13,8 @@
 
 #include <vector>
 
+#include "core_ops.h"
+
 #define HIP_CHECK(expr)                                                    \
   do {                                                                     \
     hipError_t _e = (expr);                                                \
@@ -805,4 +807,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("shallow_mfma_fwd", &shallow_mfma_fwd);
   m.def("shallow_mask_convert", &shallow_mask_convert);
   m.def("shallow_mfma_bwd", &shallow_mfma_bwd);
+  register_core_ops(m);
 }
