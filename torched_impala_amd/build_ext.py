@@ -78,10 +78,11 @@ def build_actor(force: bool = False) -> str:
 HIP_SOURCES = ["hip_ext.cpp", "vtrace_kernels.hip", "lstm_kernels.hip",
                "optim_kernels.hip", "conv_kernels.hip", "linear_kernels.hip",
                "deep_kernels.hip", "shallow_mfma.hip", "shallow_mfma_bwd.hip",
-               "pack_kernels.hip", "core_ops.cpp", "norm_kernels.hip"]
+               "pack_kernels.hip", "core_ops.cpp", "norm_kernels.hip",
+               "attn_kernels.hip"]
 
 
-HIP_HEADERS = ["core_ops.h"]
+HIP_HEADERS = ["core_ops.h", "attn_kernels.h"]
 
 
 def build_probe(force: bool = False) -> str:
