@@ -128,18 +128,17 @@ struct DeviceScope {
 // transport: arenas are plain shm; the learner page-locks its mapping so
 // hipMemcpyAsync drains are real async DMA).
 // ---------------------------------------------------------------------------
-void host_register(torch::Tensor t) {
+// false: the driver does not page-lock this memory (some hosts refuse any
+// that already exists); copies still work, staged by the runtime
+bool host_register(torch::Tensor t) {
   TORCH_CHECK(!t.is_cuda(), "host_register takes a CPU tensor");
   TORCH_CHECK(t.is_contiguous(), "must be contiguous");
   void* ptr = t.data_ptr();
   size_t bytes = t.numel() * t.element_size();
   hipError_t e = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
-  if (e == hipErrorHostMemoryAlreadyRegistered) {
-    (void)hipGetLastError();
-    return;
-  }
-  TORCH_CHECK(e == hipSuccess, "hipHostRegister failed: ",
-              hipGetErrorString(e));
+  // the error is not left behind for the next call to report
+  if (e != hipSuccess) (void)hipGetLastError();
+  return e == hipSuccess || e == hipErrorHostMemoryAlreadyRegistered;
 }
 
 void host_unregister(torch::Tensor t) {

@@ -62,11 +62,16 @@ def hip_available() -> bool:
 
 
 def pin_host_memory(t: torch.Tensor):
-    """hipHostRegister a CPU tensor's storage (page-lock for async DMA)."""
+    """hipHostRegister a CPU tensor's storage (page-lock for async DMA).
+
+    Where the driver refuses, the tensor stays pageable: copies from and to
+    it are still ordered on their stream, only slower."""
     ext = ext_hip(required=True)
     if ext is None:
         return
-    ext.host_register(t)
+    if not ext.host_register(t):
+        log.warning("the driver refused to page-lock %d bytes; copies go "
+                    "through pageable memory", t.numel() * t.element_size())
 
 
 def unpin_host_memory(t: torch.Tensor):
