@@ -1,0 +1,269 @@
+"""Newton-Schulz orthogonalisation against its definition in 64 bits.
+
+Tolerances come from the arithmetic, not from a run. A product of a round is
+computed from operands of 22 bits with fp32 sums: with u = 2^-22 its relative
+error, in the Frobenius norm of the product's magnitudes, stays under 4 u
+(operands, dropped low product, sums). An error of X in one round is carried
+on by the later ones: the derivative of p(s) = a s + b s^3 + c s^5 on [0,
+1.21] is at most a = 3.4445 in magnitude, and so is that of the matrix map
+between two singular directions up to a factor of 2. So an error e_k of round
+k's X (its norm times 4 u for each of three products, the middle one weighted
+by |b| + 2 |c| < 10) gives at most 2 a^(steps - k) e_k in the result:
+
+    |error|_F <= sum_k 2 a^(steps-k) * 48 u * |X_k|_F,   |X_k|_F <= a^k, sqrt(m) * 1.21
+"""
+import math
+
+import pytest
+import torch
+
+from torched_impala_amd.ops.orthogonal import COEFFICIENTS, orthogonalize
+
+A, B, C = COEFFICIENTS
+U22 = 2.0 ** -22
+
+
+def _ref(g, steps=5, eps=1e-7):
+    x = g.detach().double().cpu()
+    x = x / (torch.linalg.vector_norm(x) + eps)
+    if x.shape[0] <= x.shape[1]:
+        for _ in range(steps):
+            m = x @ x.T
+            x = A * x + B * (m @ x) + C * (m @ (m @ x))
+    else:
+        for _ in range(steps):
+            m = x.T @ x
+            x = A * x + B * (x @ m) + C * ((x @ m) @ m)
+    return x
+
+
+def _tol(g, steps, rho=1.0):
+    m = min(g.shape)
+    return sum(2 * A ** (steps - k) * 48 * U22
+               * min(rho * A ** k, 1.21 * math.sqrt(m))
+               for k in range(steps + 1))
+
+
+def _check(mats, steps=5, eps=1e-7, out=None):
+    got = orthogonalize(mats, steps=steps, eps=eps, out=out)
+    for g, o in zip(mats, got):
+        r = _ref(g, steps, eps)
+        assert o.shape == g.shape and o.dtype is g.dtype
+        norm = float(torch.linalg.vector_norm(g.detach().double()))
+        rho = norm / (norm + eps) if norm + eps else 0.0
+        half = torch.finfo(o.dtype).eps / 2
+        err = float(torch.linalg.vector_norm(o.double().cpu() - r))
+        # sizes under the type's smallest normal round by its step there
+        tiny = torch.finfo(o.dtype).tiny * half * 2 * math.sqrt(r.numel())
+        lim = _tol(g, steps, rho) + half * float(
+            torch.linalg.vector_norm(r)) + tiny
+        assert err <= lim, (tuple(g.shape), err, lim)
+    return got
+
+
+def _rand(m, n, dtype=torch.float32, device="cuda", seed=0, scale=1e-3):
+    gen = torch.Generator().manual_seed(seed * 1000 + m * 7 + n)
+    return (scale * torch.randn(m, n, generator=gen)).to(dtype).to(device)
+
+
+# --------------------------------------------------------------- CPU
+def test_cpu_path():
+    _check([_rand(7, 19, device="cpu"), _rand(19, 7, device="cpu"),
+            _rand(8, 8, torch.bfloat16, device="cpu")])
+    assert orthogonalize([]) == []
+    buf = [_rand(5, 6, device="cpu")]
+    ref = orthogonalize(buf)
+    assert orthogonalize(buf, out=buf)[0] is buf[0]
+    assert torch.equal(buf[0], ref[0])
+
+
+def test_singular_values_near_one():
+    g = _rand(24, 60, device="cpu", scale=1.0)
+    s = torch.linalg.svdvals(orthogonalize([g])[0])
+    assert float(s.max()) <= 1.21 and float(s.min()) >= 0.6
+
+
+def _refuse(device):
+    g = _rand(6, 8, device=device)
+    for exc, args, kw in [
+            (TypeError, [g.double()], {}),
+            (TypeError, [g.long()], {}),
+            (ValueError, [g[0]], {}),
+            (ValueError, [g[None]], {}),
+            (ValueError, [g], dict(steps=0)),
+            (ValueError, [g], dict(steps=2.5)),
+            (ValueError, [g], dict(eps=-1.0)),
+            (ValueError, [g], dict(eps=float("inf"))),
+            (ValueError, [g, g.to("meta")], {}),
+            (ValueError, [torch.empty(1 << 20, 1, device="meta")], {}),
+            (ValueError, [torch.empty(32769, 32769, device="meta")], {}),
+            (RuntimeError, [g.clone().requires_grad_()], {}),
+            (ValueError, [g], dict(out=[])),
+            (TypeError, [g], dict(out=[g.double()])),
+            (ValueError, [g], dict(out=[g[:5]])),
+            (ValueError, [g], dict(out=[torch.empty(6, 16, device=device)
+                                        [:, ::2]])),
+            (ValueError, [g], dict(out=[g[:1].expand(6, 8)])),
+            (RuntimeError, [g], dict(out=[torch.empty_like(
+                g, requires_grad=True)]))]:
+        with pytest.raises(exc):
+            orthogonalize(args, **kw)
+    pool = torch.randn(200, device=device)
+    a, b = pool[:48].view(6, 8), pool[40:88].view(6, 8)
+    with pytest.raises(ValueError):      # two results on one memory
+        orthogonalize([g, g], out=[a, b])
+    with pytest.raises(ValueError):      # a result on another's matrix
+        orthogonalize([a, g], out=[torch.empty_like(a), b])
+
+
+def test_refusals_cpu():
+    _refuse("cpu")
+
+
+# --------------------------------------------------------------- GPU
+@pytest.mark.gpu
+def test_refusals_gpu():
+    _refuse("cuda")
+
+
+SHAPES = [(1, 1), (1, 7), (7, 1), (2, 300), (16, 256), (63, 65), (64, 64),
+          (65, 63), (128, 128), (129, 127), (200, 333), (256, 1568),
+          (1024, 263), (1024, 256), (32, 288), (300, 4), (5, 5000),
+          (640, 640)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16,
+                                   torch.float16])
+def test_shapes(shape, dtype):
+    _check([_rand(*shape, dtype)])
+
+
+@pytest.mark.gpu
+def test_list_of_many():
+    """More matrices than one launch takes, all types, empty ones among."""
+    types = [torch.float32, torch.bfloat16, torch.float16]
+    mats = [_rand(3 + 5 * i, 200 - 3 * i, types[i % 3]) for i in range(60)]
+    mats[4] = mats[4][:0]
+    mats[31] = mats[31][:, :0]
+    got = _check(mats)
+    for i in (0, 7, 59):   # and each equals its own call
+        assert torch.allclose(got[i].float(),
+                              orthogonalize([mats[i]])[0].float(),
+                              atol=2 ** -8)
+
+
+@pytest.mark.gpu
+def test_wide_tiles():
+    _check([_rand(1024, 1024), _rand(2000, 1030), _rand(1030, 2000,
+                                                        torch.bfloat16),
+            _rand(33, 70)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("steps", [1, 2, 3, 8])
+def test_steps(steps):
+    _check([_rand(70, 200), _rand(200, 70)], steps=steps)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-36, 1e-20, 1e-12, 1e-8, 1e-6, 1.0, 1e6,
+                                   1e18, 1e36])
+def test_scales(scale):
+    """Any gradient's scale: norms that overflow 32 bits when squared, and
+    norms that eps outweighs, where the result stays as small as it is."""
+    _check([_rand(48, 130, scale=scale)])
+    _check([_rand(48, 130, scale=scale)], eps=0.0)
+
+
+@pytest.mark.gpu
+def test_low_rank_and_zero():
+    u, v = _rand(90, 3, scale=1.0), _rand(3, 150, scale=1.0)
+    _check([u @ v, torch.zeros(40, 70, device="cuda")])
+    assert not orthogonalize([torch.zeros(9, 9, device="cuda")])[0].any()
+    assert orthogonalize([torch.zeros(3, 3, device="cuda")],
+                         eps=0.0)[0].isnan().all()
+
+
+@pytest.mark.gpu
+def test_non_finite_stays_in_its_matrix():
+    a, b = _rand(70, 70), _rand(70, 90)
+    clean = orthogonalize([a, b])
+    for value in (float("nan"), float("inf")):
+        bad = a.clone()
+        bad[3, 4] = value
+        got = orthogonalize([bad, b])
+        assert not got[0].isfinite().any()
+        assert torch.equal(got[1], clean[1])
+
+
+@pytest.mark.gpu
+def test_strides():
+    base = torch.randn(70, 400, device="cuda")
+    mats = [base[:, :130], base[:, 1:300:3], base.t()[5:90], base[::2, 7:],
+            base[:1].expand(20, 400)]
+    got = _check(mats)
+    assert all(o.is_contiguous() for o in got)
+    # results in a larger buffer: what lies around them stays
+    pool = torch.randn(1000, device="cuda")
+    before = pool.clone()
+    out = [pool[100:100 + 210].view(14, 15), pool[400:400 + 210].view(15, 14)
+           .t()]
+    mats = [_rand(14, 15), _rand(14, 15, seed=1)]
+    orthogonalize(mats, out=out)
+    ref = orthogonalize(mats)
+    assert torch.equal(out[0], ref[0]) and torch.equal(out[1], ref[1])
+    assert torch.equal(pool[:100], before[:100])
+    assert torch.equal(pool[310:400], before[310:400])
+    assert torch.equal(pool[610:], before[610:])
+
+
+@pytest.mark.gpu
+def test_in_place():
+    mats = [_rand(70, 200), _rand(300, 40)]
+    ref = orthogonalize(mats)
+    got = orthogonalize(mats, out=mats)
+    assert got[0] is mats[0]
+    for a, b in zip(got, ref):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_repeatable_streams_and_two_at_once():
+    one = [_rand(256, 1568), _rand(1024, 256)]
+    two = [_rand(256, 1568, seed=2), _rand(1024, 256, seed=2)]
+    r1, r2 = orthogonalize(one), orthogonalize(two)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for s in (s1, s2):
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(s1):
+            g1 = orthogonalize(one)
+        with torch.cuda.stream(s2):
+            g2 = orthogonalize(two)
+        torch.cuda.synchronize()
+        for a, b in zip(r1 + r2, g1 + g2):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_captured():
+    mats = [_rand(256, 1568), _rand(1024, 263), _rand(16, 256)]
+    buf = [m.clone() for m in mats]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        orthogonalize(buf)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = orthogonalize(buf)
+    for seed in (4, 5, 6):
+        new = [_rand(*m.shape, seed=seed) for m in mats]
+        for b, n in zip(buf, new):
+            b.copy_(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(res, orthogonalize(new)):
+            assert torch.equal(a, b)

@@ -79,10 +79,10 @@ HIP_SOURCES = ["hip_ext.cpp", "vtrace_kernels.hip", "lstm_kernels.hip",
                "optim_kernels.hip", "conv_kernels.hip", "linear_kernels.hip",
                "deep_kernels.hip", "shallow_mfma.hip", "shallow_mfma_bwd.hip",
                "pack_kernels.hip", "core_ops.cpp", "norm_kernels.hip",
-               "attn_kernels.hip"]
+               "attn_kernels.hip", "ortho_kernels.hip"]
 
 
-HIP_HEADERS = ["core_ops.h", "attn_kernels.h"]
+HIP_HEADERS = ["core_ops.h", "attn_kernels.h", "ortho_kernels.h"]
 
 
 def build_probe(force: bool = False) -> str:

@@ -10,10 +10,12 @@
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <vector>
 
 #include "attn_kernels.h"
 #include "core_ops.h"
+#include "ortho_kernels.h"
 
 extern "C" {
 long layer_norm_part_elems(int, long, long, int);
@@ -31,6 +33,8 @@ void launch_attn_scan(float*, const float*, const float*, long, long, int,
                       int, hipStream_t);
 void launch_attn_step(int, const impala::attn::AttnStepArgs*, int,
                       hipStream_t);
+void launch_ns_start(impala::ortho::Args*, hipStream_t);
+void launch_ns_product(int, int, const impala::ortho::Args*, hipStream_t);
 }
 
 namespace {
@@ -473,9 +477,156 @@ Tensor linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor g,
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// Newton-Schulz orthogonalisation of lists of matrices
+// ---------------------------------------------------------------------------
+namespace ns = impala::ortho;
+
+// exponent that brings entries of 1 / sqrt(n) to about 8
+int scale_exp(long n) {
+  const int e = 3 + (int)std::lround(0.5 * std::log2((double)n));
+  return e < 13 ? e : 13;
+}
+
+// tiles of one product of one matrix, and the blocks that share a tile's k
+void plan_product(ns::Args& a, int mode, int tile) {
+  const int ks = tile == 64 ? 64 : 32;
+  long total = 0;
+  for (int i = 0; i < a.count; ++i) {
+    ns::Mat& m = a.mat[i];
+    const int tm = m.mp / tile, tn = m.np / tile;
+    m.tiles = mode == 2 ? tm * tn : tm * (tm + 1) / 2;
+    total += m.tiles;
+  }
+  int blocks = 0;
+  for (int i = 0; i < a.count; ++i) {
+    ns::Mat& m = a.mat[i];
+    // two blocks a CU fit; a block keeps 256 values of k at least, so that
+    // adding the parts does not outweigh them
+    const long steps = (mode == 0 ? m.np : m.mp) / ks;
+    long s = total >= 512 ? 1 : 512 / total;
+    const long most = steps * ks / 256;
+    if (s > most) s = most;
+    m.splits = (int)(s < 1 ? 1 : s);
+    a.first[i] = blocks;
+    blocks += m.tiles * m.splits;
+  }
+  a.first[a.count] = blocks;
+}
+
+void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
+                   long steps, double eps) {
+  TORCH_CHECK(src.size() == dst.size() && steps >= 1 && eps >= 0.0,
+              "orthogonalize: bad arguments");
+  for (size_t i = 0; i < src.size(); ++i) {
+    const Tensor &s = src[i], &d = dst[i];
+    TORCH_CHECK(s.is_cuda() && s.dim() == 2 && d.sizes() == s.sizes() &&
+                    s.device() == src[0].device() &&
+                    d.device() == s.device() &&
+                    d.scalar_type() == s.scalar_type(),
+                "orthogonalize: matrices and results must match");
+    TORCH_CHECK(s.size(0) < (1 << 20) && s.size(1) < (1 << 20) &&
+                    std::min(s.size(0), s.size(1)) <= 32768,
+                "orthogonalize: matrix too large");
+    type_code(s, "matrix");
+  }
+  size_t at = 0;
+  while (at < src.size()) {
+    ns::Args a{};
+    std::vector<size_t> take;
+    long tiles128 = 0;
+    for (; at < src.size() && take.size() < ns::MAX_MATS; ++at) {
+      if (src[at].numel() == 0) continue;
+      take.push_back(at);
+      tiles128 += ((src[at].size(0) + 127) / 128) *
+                  ((src[at].size(1) + 127) / 128);
+    }
+    if (take.empty()) break;
+    const Tensor& like = src[take[0]];
+    const c10::DeviceGuard guard(like.device());
+    hipStream_t stream = stream_here();
+    // a tile of 128 needs half the reads of 64, if there are enough of them
+    const int tile = tiles128 >= 256 ? 128 : 64;
+    a.count = (int)take.size();
+    long parts = 0;
+    for (int i = 0; i < a.count; ++i) {
+      const Tensor &s = src[take[i]], &d = dst[take[i]];
+      ns::Mat& m = a.mat[i];
+      const bool tall = s.size(0) > s.size(1);
+      const int r = tall ? 1 : 0, c = tall ? 0 : 1;
+      m.src = s.data_ptr();
+      m.src_i = s.stride(r);
+      m.src_j = s.stride(c);
+      m.dst = d.data_ptr();
+      m.dst_i = d.stride(r);
+      m.dst_j = d.stride(c);
+      m.type = type_code(s, "matrix");
+      m.m = (int)s.size(r);
+      m.n = (int)s.size(c);
+      m.mp = (m.m + tile - 1) / tile * tile;
+      m.np = (m.n + tile - 1) / tile * tile;
+      m.ex = scale_exp(m.n);
+      m.ea = scale_exp(m.m);
+      const long wide = 2L * m.mp * m.np, square = 2L * m.mp * m.mp;
+      m.x = parts;
+      m.xt[0] = m.x + wide;
+      m.xt[1] = m.xt[0] + wide;
+      m.a = m.xt[1] + wide;
+      m.b = m.a + square;
+      parts = m.b + square;
+    }
+    long partial = 1, arrived = 1;
+    for (int mode = 0; mode < 3; ++mode) {
+      plan_product(a, mode, tile);
+      long p = 0, n = 0;
+      for (int i = 0; i < a.count; ++i) {
+        n += a.mat[i].tiles;
+        if (a.mat[i].splits > 1)
+          p += (long)a.mat[i].tiles * a.mat[i].splits * tile * tile;
+      }
+      partial = p > partial ? p : partial;
+      arrived = n > arrived ? n : arrived;
+    }
+    auto work = torch::empty({parts}, like.options().dtype(torch::kFloat16));
+    auto split = torch::empty({partial},
+                              like.options().dtype(torch::kFloat32));
+    auto count = torch::zeros({arrived}, like.options().dtype(torch::kInt32));
+    auto sums = torch::empty({(long)a.count * ns::NORM_BLOCKS},
+                             like.options().dtype(torch::kFloat64));
+    auto rho = torch::empty({a.count}, like.options().dtype(torch::kFloat32));
+    a.parts = (_Float16*)work.data_ptr();
+    a.partial = split.data_ptr<float>();
+    a.arrived = count.data_ptr<int>();
+    a.sums = sums.data_ptr<double>();
+    a.rho = rho.data_ptr<float>();
+    a.eps = eps;
+    launch_ns_start(&a, stream);
+    for (long k = 0; k < steps; ++k) {
+      a.round = (int)k;
+      a.last = k + 1 == steps;
+      for (int mode = 0; mode < 3; ++mode) {
+        plan_product(a, mode, tile);
+        long p = 0;
+        int n = 0;
+        for (int i = 0; i < a.count; ++i) {
+          a.part_off[i] = p;
+          a.arrive_off[i] = n;
+          n += a.mat[i].tiles;
+          if (a.mat[i].splits > 1)
+            p += (long)a.mat[i].tiles * a.mat[i].splits * tile * tile;
+        }
+        launch_ns_product(mode, tile, &a, stream);
+      }
+    }
+    check_launch("orthogonalize");
+  }
+}
+
 }  // namespace
 
 void register_core_ops(pybind11::module_& m) {
+  m.def("orthogonalize", &orthogonalize, py::arg("src"), py::arg("dst"),
+        py::arg("steps"), py::arg("eps"));
   m.def("linear_attention_fwd", &linear_attention_fwd, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("done"),
         py::arg("state"), py::arg("scale"));

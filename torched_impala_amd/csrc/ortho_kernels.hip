@@ -1,0 +1,408 @@
+// Orthogonalised updates by Newton-Schulz products, for lists of matrices.
+//
+//   X = G / (|G| + eps);   5 times:  A = X X^T
+//                                    B = a I + b A + c A A
+//                                    X = B X
+//
+// a, b, c take singular values in (0, 1] into a band around 1 and never
+// above 1.21, so X is bounded all along. A tall matrix is worked on turned.
+//
+// Bound: matrix products for wide layers, latency for the small matrices of
+// the policy nets, so one launch does one product of all matrices of a list
+// (two launches to start, three a round).
+//
+// The products run on the fp16 matrix cores with fp32 accuracy: an operand is
+// kept as two fp16 parts, hi + lo = 22 bits, and a product is hi hi + hi lo +
+// lo hi. Rounding X to 16 bits would not do: errors in directions of small
+// singular values grow by a = 3.44 a round, 485 times in five. Powers of two
+// keep the parts in the range of fp16: X is bounded by beta_k (|G| / (|G| +
+// eps), times a each round, up to 1.25), so its entries are of the order of
+// beta_k / sqrt(n), and those of A of beta_k^2 / sqrt(m).
+//
+// A and B are symmetric: only tiles on and under the diagonal are computed,
+// and written twice. X is kept in both orientations, so that every product
+// reads both operands along k.
+
+#include <hip/hip_runtime.h>
+
+#include "ortho_kernels.h"
+
+namespace impala {
+namespace ortho {
+
+typedef _Float16 half_t;
+typedef __bf16 bf16_t;
+typedef half_t halfx8 __attribute__((ext_vector_type(8)));
+typedef half_t halfx4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
+
+__device__ inline float load_any(const void* p, long i, int type) {
+  if (type == 0) return ((const float*)p)[i];
+  if (type == 1) return (float)((const bf16_t*)p)[i];
+  return (float)((const half_t*)p)[i];
+}
+
+__device__ inline void store_any(void* p, long i, int type, float v) {
+  if (type == 0) ((float*)p)[i] = v;
+  else if (type == 1) ((bf16_t*)p)[i] = (bf16_t)v;
+  else ((half_t*)p)[i] = (half_t)v;
+}
+
+__device__ inline int mat_of(const Args& a, int block) {
+  int i = 0;
+  while (i + 1 < a.count && block >= a.first[i + 1]) ++i;
+  return i;
+}
+
+// exponent of the power of two at or below the bound of |X| in round k
+__device__ inline int bound_exp(float rho, int k) {
+  float beta = rho;
+  for (int i = 0; i < k; ++i) beta = fminf(1.25f, 3.4445f * beta);
+  if (!(beta > 1e-30f)) return -100;   // zero: any scale does; NaN too
+  int e;
+  frexpf(beta, &e);
+  return e - 1;
+}
+
+__device__ inline double block_sum(double v) {
+  __shared__ double s[4];
+  for (int off = 32; off > 0; off >>= 1) v += __shfl_down(v, off, 64);
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return s[0] + s[1] + s[2] + s[3];
+}
+
+// sums of squares in 64 bits: no overflow for any fp32 gradient, and an order
+// of adding that does not change
+__global__ void __launch_bounds__(256) ns_norm(Args args) {
+  const int mi = blockIdx.x / NORM_BLOCKS, blk = blockIdx.x % NORM_BLOCKS;
+  const Mat& M = args.mat[mi];
+  const long total = (long)M.m * M.n;
+  // the axis that is contiguous in memory runs fastest
+  const bool by_i = M.src_i < M.src_j;
+  const int fast = by_i ? M.m : M.n;
+  const long sf = by_i ? M.src_i : M.src_j, ss = by_i ? M.src_j : M.src_i;
+  double acc = 0.0;
+  for (long e = (long)blk * 256 + threadIdx.x; e < total;
+       e += (long)NORM_BLOCKS * 256) {
+    const long s = e / fast, f = e - s * fast;
+    const double v = load_any(M.src, s * ss + f * sf, M.type);
+    acc += v * v;
+  }
+  acc = block_sum(acc);
+  if (threadIdx.x == 0) args.sums[mi * NORM_BLOCKS + blk] = acc;
+}
+
+__device__ inline void split_store(half_t* p, long plane, long at, float v) {
+  const half_t h = (half_t)v;
+  p[at] = h;
+  p[at + plane] = (half_t)(v - (float)h);
+}
+
+// G -> parts of X and X^T, 64 x 64 a block
+__global__ void __launch_bounds__(256) ns_prepare(Args args) {
+  __shared__ float tile[64][65];
+  const int mi = mat_of(args, blockIdx.x);
+  const Mat& M = args.mat[mi];
+  const int t = blockIdx.x - args.first[mi];
+  const int tn = M.np / 64;
+  const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
+
+  double sum = 0.0;
+  for (int k = 0; k < NORM_BLOCKS; ++k) sum += args.sums[mi * NORM_BLOCKS + k];
+  const double norm = sqrt(sum);
+  const float rho = (float)(norm / (norm + args.eps));
+  const int e = M.ex - bound_exp(rho, 0);
+  const double mul = ldexp(1.0 / (norm + args.eps), e);
+  if (t == 0 && threadIdx.x == 0) args.rho[mi] = rho;
+
+  const bool by_i = M.src_i < M.src_j;
+  #pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int f = threadIdx.x & 63, s = (threadIdx.x >> 6) + 4 * k;
+    const int i = by_i ? f : s, j = by_i ? s : f;
+    float v = 0.f;
+    if (i0 + i < M.m && j0 + j < M.n)
+      v = (float)(mul * (double)load_any(M.src, (i0 + i) * M.src_i +
+                                                    (j0 + j) * M.src_j,
+                                         M.type));
+    tile[i][j] = v;
+  }
+  __syncthreads();
+  const long plane = (long)M.mp * M.np;
+  half_t* x = args.parts + M.x;
+  half_t* xt = args.parts + M.xt[0];
+  #pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const int f = threadIdx.x & 63, s = (threadIdx.x >> 6) + 4 * k;
+    split_store(x, plane, (long)(i0 + s) * M.np + j0 + f, tile[s][f]);
+    split_store(xt, plane, (long)(j0 + s) * M.mp + i0 + f, tile[f][s]);
+  }
+}
+
+// --------------------------------------------------------------------------
+// One product, C = P Q^T over k, P and Q in two parts with k contiguous.
+// MODE 0: A = X X^T. MODE 1: B = a I + b A + c A A. MODE 2: X = B X.
+// TILE x TILE of C a block, four waves of half that each way; k in steps of
+// KS through two LDS buffers, the next step's rows on their way in registers.
+// Few tiles of long k are split; the last block of a tile to arrive adds the
+// parts, in order.
+// --------------------------------------------------------------------------
+template <int MODE, int TILE>
+__global__ void __launch_bounds__(256) ns_product(Args args) {
+  constexpr int KS = TILE == 64 ? 64 : 32;
+  constexpr int LD = KS + 8;              // rows 4 banks apart
+  constexpr int W = TILE / 2, NF = W / 16;
+  constexpr int PIECES = TILE * KS / 8 / 256;   // 16-byte pieces a thread
+  constexpr int PER_ROW = KS / 8;
+  __shared__ __align__(16) half_t lds[2][4][TILE * LD];
+
+  const int mi = mat_of(args, blockIdx.x);
+  const Mat& M = args.mat[mi];
+  const int id = blockIdx.x - args.first[mi];
+  const int tile = id / M.splits, split = id % M.splits;
+  int ti, tj;
+  if (MODE == 2) {
+    const int tn = M.np / TILE;
+    ti = tile / tn;
+    tj = tile % tn;
+  } else {   // under the diagonal, row by row
+    ti = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
+    while (ti * (ti + 1) / 2 > tile) --ti;
+    tj = tile - ti * (ti + 1) / 2;
+  }
+  const int cur = args.round & 1;
+  const int K = MODE == 0 ? M.np : M.mp;
+  const long plane_p = MODE == 0 ? (long)M.mp * M.np : (long)M.mp * M.mp;
+  const long plane_q = MODE == 1 ? (long)M.mp * M.mp : (long)M.mp * M.np;
+  const half_t* P = args.parts + (MODE == 0 ? M.x : MODE == 1 ? M.a : M.b) +
+                    (long)ti * TILE * K;
+  const half_t* Q =
+      args.parts + (MODE == 0 ? M.x : MODE == 1 ? M.a : M.xt[cur]) +
+      (long)tj * TILE * K;
+
+  const int tid = threadIdx.x, l = tid & 63, m = l & 15, g = l >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wi = (wave >> 1) * W, wj = (wave & 1) * W;
+
+  const int steps = K / KS;
+  const int per = (steps + M.splits - 1) / M.splits;
+  const int k_lo = split * per;
+  const int k_hi = k_lo + per < steps ? k_lo + per : steps;
+
+  u32x4 r0[PIECES], r1[PIECES], r2[PIECES], r3[PIECES];
+  auto fetch = [&](int step) __attribute__((always_inline)) {
+    #pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+      const int idx = n * 256 + tid;
+      const long off =
+          (long)(idx / PER_ROW) * K + step * KS + (idx % PER_ROW) * 8;
+      r0[n] = *reinterpret_cast<const u32x4*>(P + off);
+      r1[n] = *reinterpret_cast<const u32x4*>(P + plane_p + off);
+      r2[n] = *reinterpret_cast<const u32x4*>(Q + off);
+      r3[n] = *reinterpret_cast<const u32x4*>(Q + plane_q + off);
+    }
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    #pragma unroll
+    for (int n = 0; n < PIECES; ++n) {
+      const int idx = n * 256 + tid;
+      const int at = (idx / PER_ROW) * LD + (idx % PER_ROW) * 8;
+      *reinterpret_cast<u32x4*>(&lds[buf][0][at]) = r0[n];
+      *reinterpret_cast<u32x4*>(&lds[buf][1][at]) = r1[n];
+      *reinterpret_cast<u32x4*>(&lds[buf][2][at]) = r2[n];
+      *reinterpret_cast<u32x4*>(&lds[buf][3][at]) = r3[n];
+    }
+  };
+
+  f32x4 acc[NF][NF];
+  #pragma unroll
+  for (int i = 0; i < NF; ++i) {
+    #pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  if (k_lo < k_hi) {
+    fetch(k_lo);
+    put(0);
+  }
+  for (int k = k_lo; k < k_hi; ++k) {
+    const int buf = (k - k_lo) & 1;
+    __syncthreads();
+    if (k + 1 < k_hi) fetch(k + 1);
+    #pragma unroll
+    for (int s = 0; s < KS / 32; ++s) {
+      halfx8 ph[NF], pl[NF], qh[NF], ql[NF];
+      #pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        const int pa = (wi + 16 * i + m) * LD + 32 * s + 8 * g;
+        const int qa = (wj + 16 * i + m) * LD + 32 * s + 8 * g;
+        ph[i] = *reinterpret_cast<const halfx8*>(&lds[buf][0][pa]);
+        pl[i] = *reinterpret_cast<const halfx8*>(&lds[buf][1][pa]);
+        qh[i] = *reinterpret_cast<const halfx8*>(&lds[buf][2][qa]);
+        ql[i] = *reinterpret_cast<const halfx8*>(&lds[buf][3][qa]);
+      }
+      #pragma unroll
+      for (int i = 0; i < NF; ++i) {
+        #pragma unroll
+        for (int j = 0; j < NF; ++j) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              ph[i], qh[j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              ph[i], ql[j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              pl[i], qh[j], acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+    if (k + 1 < k_hi) put(buf ^ 1);
+  }
+
+  if (M.splits > 1) {
+    // leave the part; whoever comes last adds all of the tile
+    float* base = args.partial + args.part_off[mi] +
+                  (long)tile * M.splits * TILE * TILE;
+    float* mine = base + (long)split * TILE * TILE;
+    #pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      #pragma unroll
+      for (int j = 0; j < NF; ++j)
+        *reinterpret_cast<f32x4*>(mine + ((i * NF + j) * 256 + tid) * 4) =
+            acc[i][j];
+    }
+    __threadfence();
+    __syncthreads();
+    int* count = args.arrived + args.arrive_off[mi] + tile;
+    // the flag lies in the operands' LDS, which is free by now: two blocks of
+    // 128 x 128 fill a CU's 160 KB to the byte
+    int* last_block = reinterpret_cast<int*>(&lds[0][0][0]);
+    if (tid == 0)
+      *last_block = __hip_atomic_fetch_add(count, 1, __ATOMIC_ACQ_REL,
+                                           __HIP_MEMORY_SCOPE_AGENT) ==
+                    M.splits - 1;
+    __syncthreads();
+    if (!*last_block) return;
+    __threadfence();
+    #pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      #pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < M.splits; ++s)
+          sum += *reinterpret_cast<const f32x4*>(
+              base + (long)s * TILE * TILE + ((i * NF + j) * 256 + tid) * 4);
+        acc[i][j] = sum;
+      }
+    }
+    if (tid == 0)   // ready for the next launch
+      __hip_atomic_store(count, 0, __ATOMIC_RELAXED,
+                         __HIP_MEMORY_SCOPE_AGENT);
+  }
+
+  // ---- scales, the polynomial, both orientations
+  const float rho = args.rho[mi];
+  const int e_now = bound_exp(rho, args.round);
+  const int sx = M.ex - e_now;               // X   = stored * 2^-sx
+  const int sa = M.ea - 2 * e_now;           // A   = stored * 2^-sa
+  const int sb = M.ea;                       // B   = stored * 2^-sb
+  const int sx2 = M.ex - bound_exp(rho, args.round + 1);
+  half_t* C = args.parts + (MODE == 0 ? M.a : MODE == 1 ? M.b : M.x);
+  half_t* CT = MODE == 2 ? args.parts + M.xt[cur ^ 1] : C;
+  const int ldc = MODE == 2 ? M.np : M.mp;
+  const long plane = MODE == 2 ? (long)M.mp * M.np : (long)M.mp * M.mp;
+  const half_t* Ap = args.parts + M.a;
+  // products of stored values -> stored values. Two factors, so that the
+  // exponents of tiny gradients stay in range
+  const float f1 = MODE == 0 ? ldexpf(1.f, sa - 2 * sx)
+                 : MODE == 1 ? ldexpf(NS_C, -2 * M.ea)
+                             : args.last ? ldexpf(1.f, -sb)
+                                         : ldexpf(1.f, sx2 - sb - sx);
+  const float f2 = MODE == 1 ? ldexpf(1.f, 4 * e_now + sb)
+                 : MODE == 2 && args.last ? ldexpf(1.f, -sx) : 1.f;
+  const float fb = ldexpf(NS_B, -M.ea + 2 * e_now + sb);
+  const float fa = ldexpf(NS_A, sb);
+
+  #pragma unroll
+  for (int i = 0; i < NF; ++i) {
+    #pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const int row = ti * TILE + wi + 16 * i + 4 * g;   // + r
+      const int col = tj * TILE + wj + 16 * j + m;
+      float v[4];
+      #pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) v[r4] = acc[i][j][r4] * f1 * f2;
+      if constexpr (MODE == 1) {
+        #pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const long at = (long)(row + r4) * ldc + col;
+          v[r4] = fmaf(fb, (float)Ap[at] + (float)Ap[at + plane], v[r4]);
+          if (row + r4 == col) v[r4] += fa;
+        }
+      }
+      if (MODE == 2 && args.last) {
+        #pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+          if (row + r4 < M.m && col < M.n)
+            store_any(M.dst, (row + r4) * M.dst_i + col * M.dst_j, M.type,
+                      v[r4]);
+        continue;
+      }
+      halfx4 h, w;
+      #pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        h[r4] = (half_t)v[r4];
+        w[r4] = (half_t)(v[r4] - (float)h[r4]);
+        const long at = (long)(row + r4) * ldc + col;
+        C[at] = h[r4];
+        C[at + plane] = w[r4];
+      }
+      if (MODE == 2 || ti != tj) {
+        const long at = (long)col * M.mp + row;
+        *reinterpret_cast<halfx4*>(CT + at) = h;
+        *reinterpret_cast<halfx4*>(CT + at + plane) = w;
+      }
+    }
+  }
+}
+
+template <int TILE>
+void run_product(int mode, const Args& a, int blocks, hipStream_t s) {
+  const dim3 grid(blocks), block(256);
+  if (mode == 0)
+    hipLaunchKernelGGL((ns_product<0, TILE>), grid, block, 0, s, a);
+  else if (mode == 1)
+    hipLaunchKernelGGL((ns_product<1, TILE>), grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL((ns_product<2, TILE>), grid, block, 0, s, a);
+}
+
+}  // namespace ortho
+}  // namespace impala
+
+using namespace impala::ortho;
+
+extern "C" {
+
+void launch_ns_start(Args* a, hipStream_t s) {
+  hipLaunchKernelGGL(ns_norm, dim3(a->count * NORM_BLOCKS), dim3(256), 0, s,
+                     *a);
+  int n = 0;
+  for (int i = 0; i < a->count; ++i) {
+    a->first[i] = n;
+    n += (a->mat[i].mp / 64) * (a->mat[i].np / 64);
+  }
+  a->first[a->count] = n;
+  hipLaunchKernelGGL(ns_prepare, dim3(n), dim3(256), 0, s, *a);
+}
+
+// the caller has set tiles, splits and first
+void launch_ns_product(int mode, int tile, const Args* a, hipStream_t s) {
+  const int blocks = a->first[a->count];
+  if (tile == 64) run_product<64>(mode, *a, blocks, s);
+  else run_product<128>(mode, *a, blocks, s);
+}
+
+}  // extern "C"
