@@ -210,7 +210,10 @@ class Rollout:
         self.fast = None
         jit_mode = getattr(flags, "actor_jit", "safe")
         use_lstm = getattr(model, "use_lstm", False)
-        if jit_mode != "off" and hasattr(model, "encode"):
+        # the fast tiers cover feedforward and LSTM policies; a
+        # linear-attention core steps eagerly
+        if (jit_mode != "off" and hasattr(model, "encode")
+                and not getattr(model, "use_linear_attention", False)):
             try:
                 if (jit_mode in ("native", "native-bf16")
                         and getattr(model, "obs_shape", None) == (4, 84, 84)):

@@ -43,6 +43,7 @@ class Flags:
 
     # --- model ---
     use_lstm: bool = False
+    use_linear_attention: bool = False  # linear-attention core instead
     model: str = "auto"                # auto | mlp | shallow | deep
 
     # --- loss / algorithm (IMPALA paper App. G canonical values) ---
@@ -62,6 +63,11 @@ class Flags:
     lambda_: float = 1.0
 
     # --- optimizer (RMSProp, paper defaults) ---
+    optimizer: str = "rmsprop"        # rmsprop | muon (matrices by
+                                      # orthogonalised momentum, the rest
+                                      # by RMSProp)
+    muon_learning_rate: float = 0.02
+    muon_momentum: float = 0.95
     learning_rate: float = 0.0006
     alpha: float = 0.99               # RMSProp smoothing
     momentum: float = 0.0
@@ -119,6 +125,7 @@ def build_parser() -> argparse.ArgumentParser:
                             "native-bf16"])
     p.add_argument("--actor-jit-refresh", type=int, default=f.actor_jit_refresh)
     _add_bool(p, "use-lstm", f.use_lstm)
+    _add_bool(p, "use-linear-attention", f.use_linear_attention)
     p.add_argument("--model", default=f.model,
                    choices=["auto", "mlp", "shallow", "deep"])
     p.add_argument("--entropy-cost", type=float, default=f.entropy_cost)
@@ -133,6 +140,11 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("--clip-pg-rho-threshold", type=float,
                    default=f.clip_pg_rho_threshold)
     p.add_argument("--lambda", dest="lambda_", type=float, default=f.lambda_)
+    p.add_argument("--optimizer", default=f.optimizer,
+                   choices=["rmsprop", "muon"])
+    p.add_argument("--muon-learning-rate", type=float,
+                   default=f.muon_learning_rate)
+    p.add_argument("--muon-momentum", type=float, default=f.muon_momentum)
     p.add_argument("--learning-rate", type=float, default=f.learning_rate)
     p.add_argument("--alpha", type=float, default=f.alpha)
     p.add_argument("--momentum", type=float, default=f.momentum)

@@ -45,6 +45,8 @@ void launch_grad_sqnorm(const float*, long, const float*, float*,
 void launch_rmsprop_update(float*, const float*, float*, long, const float*,
                            const float*, const float*, float, float, float,
                            float*, hipStream_t);
+void launch_muon_momentum(const float*, float*, float*, long, const float*,
+                          const float*, float, float, float*, hipStream_t);
 void launch_shallow_encoder_fwd(const unsigned char*, const float*,
                                 const float*, const float*, const float*,
                                 const float*, const float*, int, float*,
@@ -349,6 +351,64 @@ void fused_clip_rmsprop(torch::Tensor flat_p, torch::Tensor flat_g,
                         lr.data_ptr<float>(), norm_sq.data_ptr<float>(),
                         scale.data_ptr<float>(), (float)max_norm,
                         (float)alpha, (float)eps, skip_p, stream);
+  HIP_CHECK(hipGetLastError());
+}
+
+// the same steps one by one, for an arena that two updates share: the norm
+// over all of it (norm_sq zeroed by the caller), then each update its part
+void grad_sqnorm(torch::Tensor flat_g, torch::Tensor scale,
+                 torch::Tensor norm_sq) {
+  check_f32(flat_g, "flat_g");
+  check_f32(scale, "scale");
+  check_f32(norm_sq, "norm_sq");
+  DeviceScope guard(flat_g.get_device());
+  launch_grad_sqnorm(flat_g.data_ptr<float>(), flat_g.numel(),
+                     scale.data_ptr<float>(), norm_sq.data_ptr<float>(),
+                     current_stream());
+  HIP_CHECK(hipGetLastError());
+}
+
+void rmsprop_update(torch::Tensor flat_p, torch::Tensor flat_g,
+                    torch::Tensor flat_sqavg, torch::Tensor lr,
+                    torch::Tensor norm_sq, torch::Tensor scale,
+                    double max_norm, double alpha, double eps) {
+  check_f32(flat_p, "flat_p");
+  check_f32(flat_g, "flat_g");
+  check_f32(flat_sqavg, "flat_sqavg");
+  check_f32(lr, "lr");
+  check_f32(norm_sq, "norm_sq");
+  check_f32(scale, "scale");
+  const long n = flat_p.numel();
+  TORCH_CHECK(flat_g.numel() == n && flat_sqavg.numel() == n,
+              "parameters, gradients and averages must match");
+  DeviceScope guard(flat_p.get_device());
+  launch_rmsprop_update(flat_p.data_ptr<float>(), flat_g.data_ptr<float>(),
+                        flat_sqavg.data_ptr<float>(), n,
+                        lr.data_ptr<float>(), norm_sq.data_ptr<float>(),
+                        scale.data_ptr<float>(), (float)max_norm,
+                        (float)alpha, (float)eps, nullptr, current_stream());
+  HIP_CHECK(hipGetLastError());
+}
+
+void muon_momentum(torch::Tensor flat_g, torch::Tensor momentum,
+                   torch::Tensor update, torch::Tensor norm_sq,
+                   torch::Tensor scale, double max_norm, double mu,
+                   torch::Tensor skip_count) {
+  check_f32(flat_g, "flat_g");
+  check_f32(momentum, "momentum");
+  check_f32(update, "update");
+  check_f32(norm_sq, "norm_sq");
+  check_f32(scale, "scale");
+  check_f32(skip_count, "skip_count");
+  const long n = flat_g.numel();
+  TORCH_CHECK(n > 0 && momentum.numel() == n && update.numel() == n,
+              "gradients, momentum and update must match");
+  DeviceScope guard(flat_g.get_device());
+  launch_muon_momentum(flat_g.data_ptr<float>(), momentum.data_ptr<float>(),
+                       update.data_ptr<float>(), n,
+                       norm_sq.data_ptr<float>(), scale.data_ptr<float>(),
+                       (float)max_norm, (float)mu,
+                       skip_count.data_ptr<float>(), current_stream());
   HIP_CHECK(hipGetLastError());
 }
 
@@ -780,6 +840,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("norm_sq"), py::arg("scale"), py::arg("max_norm"),
         py::arg("alpha"), py::arg("eps"),
         py::arg("skip_count") = py::none());
+  m.def("grad_sqnorm", &grad_sqnorm);
+  m.def("rmsprop_update", &rmsprop_update);
+  m.def("muon_momentum", &muon_momentum);
   m.def("shallow_encoder_fwd", &shallow_encoder_fwd);
   m.def("shallow_encoder_bwd", &shallow_encoder_bwd);
   m.def("linear_mfma", &linear_mfma, py::arg("A"), py::arg("B"),

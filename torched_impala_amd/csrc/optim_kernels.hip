@@ -74,9 +74,48 @@ __global__ void rmsprop_update_kernel(
   }
 }
 
+// m = mu m + g;  u = g + mu m, with g clipped and scaled as above. A step
+// whose norm is not finite leaves m and gives u = 0, so that nothing behind
+// it moves.
+__global__ void muon_momentum_kernel(
+    const float* __restrict__ g, float* __restrict__ mom,
+    float* __restrict__ upd, long n, const float* __restrict__ norm_sq,
+    const float* __restrict__ scale, float max_norm, float mu,
+    float* __restrict__ skip_count) {
+  const bool ok = isfinite(norm_sq[0]);
+  if (!ok && blockIdx.x == 0 && threadIdx.x == 0 && skip_count != nullptr)
+    skip_count[0] += 1.f;
+  float cs = scale[0];
+  if (max_norm > 0.f)
+    cs *= fminf(1.f, max_norm / (sqrtf(norm_sq[0]) + 1e-6f));
+  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n;
+       i += (long)gridDim.x * blockDim.x) {
+    if (ok) {
+      const float gv = g[i] * cs;
+      const float m = fmaf(mu, mom[i], gv);
+      mom[i] = m;
+      upd[i] = fmaf(mu, m, gv);
+    } else {
+      upd[i] = 0.f;
+    }
+  }
+}
+
 }  // namespace impala
 
 extern "C" {
+
+void launch_muon_momentum(const float* g, float* mom, float* upd, long n,
+                          const float* norm_sq, const float* scale,
+                          float max_norm, float mu, float* skip_count,
+                          hipStream_t stream) {
+  const int block = 256;
+  long grid = (n + block - 1) / block;
+  if (grid > 2048) grid = 2048;
+  hipLaunchKernelGGL(impala::muon_momentum_kernel, dim3((int)grid),
+                     dim3(block), 0, stream, g, mom, upd, n, norm_sq, scale,
+                     max_norm, mu, skip_count);
+}
 
 void launch_grad_sqnorm(const float* g, long n, const float* scale,
                         float* out, hipStream_t stream) {

@@ -26,7 +26,8 @@ from torched_impala_amd.config import Flags
 from torched_impala_amd.envs import env_spec
 from torched_impala_amd.metrics import MetricsLogger, StageTimers
 from torched_impala_amd.models import build_model
-from torched_impala_amd.ops.optim import FlatRMSprop
+from torched_impala_amd.ops.optim import (FlatMuon, FlatRMSprop,
+                                          muon_matrices)
 from torched_impala_amd.parallel import (FlatGradReducer, GradReducer,
                                          init_distributed)
 from torched_impala_amd.transport import SlotQueue, TrajectoryBuffers, WeightMirror
@@ -54,7 +55,10 @@ def create_buffers(flags: Flags, obs_shape, obs_dtype, num_actions
         num_actions=num_actions,
         num_slots=num_slots,
         lstm_hidden=256 if flags.use_lstm else 0,
-        envs_per_slot=n)
+        envs_per_slot=n,
+        # 4 heads of 64 x 64 (models/core.py)
+        core_state=((1, 4 * 64 * 64) if flags.use_linear_attention
+                    else (0, 0)))
 
 
 class Batcher:
@@ -119,7 +123,7 @@ class Batcher:
 
     def next_batch(self, materialize: bool = True) -> Dict[str, torch.Tensor]:
         """Returns time-major batch: frame (T+1, B, *obs), ...,
-        initial_core_state (2, B, H) if present. With materialize=False
+        initial_core_state (parts, B, H) if present. With materialize=False
         (graph mode) only drains into the staging buffer and returns its
         index — the captured graph owns the time-major views."""
         if not self.is_cuda:
@@ -176,8 +180,9 @@ class Batcher:
                 out[key] = ext.unpack_time_major(v.contiguous(), 1)
                 continue
             if key == "initial_core_state":
-                # (k, 2, n, H) -> (2, k*n, H)
-                out[key] = v.permute(1, 0, 2, 3).reshape(2, k * n, -1)
+                # (k, parts, n, H) -> (parts, k*n, H)
+                out[key] = v.permute(1, 0, 2, 3).reshape(
+                    v.shape[1], k * n, v.shape[3])
             else:
                 # (k, T+1, n, ...) -> (T+1, k*n, ...)
                 out[key] = v.transpose(0, 1).reshape(
@@ -204,8 +209,7 @@ def _fwd_bwd(flags: Flags, model, batch: Dict[str, torch.Tensor],
     t.start("forward")
     core_state = ()
     if "initial_core_state" in batch:
-        ics = batch["initial_core_state"]
-        core_state = (ics[0], ics[1])
+        core_state = tuple(batch["initial_core_state"].unbind(0))
     inputs = dict(frame=batch["frame"], reward=batch["reward"],
                   done=batch["done"], last_action=batch["last_action"])
     if flags.compute_dtype == "bf16" and batch["frame"].is_cuda:
@@ -316,8 +320,7 @@ class GraphedStep:
         # step_device inside _fn) — snapshot the flat state so capture
         # doesn't bake in up to 2*WARMUP_ITERS uncounted weight updates
         # from the same batch
-        snap = (self.optimizer.flat_param.clone(),
-                self.optimizer.flat_sqavg.clone())
+        snap = [t.clone() for t in self.optimizer.state_arenas()]
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -325,8 +328,8 @@ class GraphedStep:
                 self._fn(i)
         torch.cuda.current_stream().wait_stream(s)
         with torch.no_grad():
-            self.optimizer.flat_param.copy_(snap[0])
-            self.optimizer.flat_sqavg.copy_(snap[1])
+            for t, was in zip(self.optimizer.state_arenas(), snap):
+                t.copy_(was)
         del snap
         g = torch.cuda.CUDAGraph()
         ctx = (torch.cuda.graph(g, pool=self.pool) if self.pool is not None
@@ -387,7 +390,19 @@ class GraphedStep:
 
 
 def build_optimizer(flags: Flags, model, world_size: int = 1):
-    if flags.momentum == 0.0:
+    if flags.optimizer == "muon":
+        if flags.momentum != 0.0:
+            raise ValueError("--momentum is RMSProp's; with --optimizer muon "
+                             "use --muon-momentum")
+        optimizer = FlatMuon(
+            model.parameters(), muon_matrices(model),
+            lr=flags.learning_rate, alpha=flags.alpha, eps=flags.epsilon,
+            max_grad_norm=flags.grad_norm_clipping, world_size=world_size,
+            muon_lr=flags.muon_learning_rate,
+            muon_momentum=flags.muon_momentum)
+    elif flags.optimizer != "rmsprop":
+        raise ValueError(f"unknown optimizer {flags.optimizer!r}")
+    elif flags.momentum == 0.0:
         optimizer = FlatRMSprop(
             model.parameters(), lr=flags.learning_rate, alpha=flags.alpha,
             eps=flags.epsilon, max_grad_norm=flags.grad_norm_clipping,
@@ -516,8 +531,8 @@ def train(flags: Flags, max_learner_steps: Optional[int] = None,
             # belt and braces: bitwise-identical start even if a rank
             # raced the file; also agree on the resume step.
             if isinstance(optimizer, FlatRMSprop):
-                torch.distributed.broadcast(optimizer.flat_param, src=0)
-                torch.distributed.broadcast(optimizer.flat_sqavg, src=0)
+                for t in optimizer.state_arenas():
+                    torch.distributed.broadcast(t, src=0)
             else:
                 for p in model.parameters():
                     torch.distributed.broadcast(p.data, src=0)

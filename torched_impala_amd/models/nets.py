@@ -5,7 +5,8 @@ the IMPALA paper, Espeholt et al. 2018):
 
 * ``MLPPolicy``    — CartPole-class: 2x64 hidden, policy + baseline heads.
 * ``ShallowNet``   — the "shallow" IMPALA net: conv 16x8x8/s4,
-  32x4x4/s2, 32x3x3/s1 -> FC-256 -> heads, optional LSTMCell(256) core.
+  32x4x4/s2, 32x3x3/s1 -> FC-256 -> heads, optional LSTMCell(256) or
+  linear-attention core (models/core.py).
 * ``DeepResNet``   — the 15-layer "deep" IMPALA net: 3 sections of
   [conv3x3 -> maxpool3x3/s2 -> 2 residual blocks] with 16/32/32 channels.
 
@@ -29,24 +30,37 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from torched_impala_amd.models.core import LinearAttentionCore
+
 
 def _flatten_time(x: torch.Tensor) -> torch.Tensor:
     return x.reshape(-1, *x.shape[2:])
 
 
 class _CoreMixin(nn.Module):
-    """LSTM-or-identity core over the unroll, with done-mask state resets."""
+    """LSTM, linear-attention or identity core over the unroll, with
+    done-mask state resets."""
 
-    def _init_core(self, core_input_size: int, use_lstm: bool, hidden: int = 256):
+    def _init_core(self, core_input_size: int, use_lstm: bool, hidden: int = 256,
+                   use_linear_attention: bool = False):
+        if use_lstm and use_linear_attention:
+            raise ValueError("a model has one core: use_lstm and "
+                             "use_linear_attention exclude each other")
         self.use_lstm = use_lstm
+        self.use_linear_attention = use_linear_attention
         self.core_input_size = core_input_size
-        if use_lstm:
+        if use_linear_attention:
+            self.core = LinearAttentionCore(core_input_size, hidden)
+            self.core_output_size = hidden
+        elif use_lstm:
             self.core = nn.LSTMCell(core_input_size, hidden)
             self.core_output_size = hidden
         else:
             self.core_output_size = core_input_size
 
     def initial_state(self, batch_size: int) -> Tuple[torch.Tensor, ...]:
+        if self.use_linear_attention:
+            return self.core.initial_state(batch_size)
         if not self.use_lstm:
             return tuple()
         p = next(self.parameters())
@@ -58,6 +72,9 @@ class _CoreMixin(nn.Module):
     def _run_core(self, core_input: torch.Tensor, done: torch.Tensor,
                   core_state: Tuple[torch.Tensor, ...]):
         """core_input: (T, B, F); done: (T, B) bool -> (T*B, out), state."""
+        if self.use_linear_attention:
+            return self.core(core_input, done, core_state,
+                             getattr(self, "force_eager_core", False))
         if not self.use_lstm:
             return _flatten_time(core_input), tuple()
         T, B = core_input.shape[:2]
@@ -115,7 +132,8 @@ def _core_extras(inputs, num_actions: int, dtype: torch.dtype):
 class MLPPolicy(_CoreMixin, _HeadsMixin):
     """CartPole-class MLP actor-critic (BASELINE.json:7)."""
 
-    def __init__(self, obs_shape=(4,), num_actions=2, use_lstm=False, hidden=64):
+    def __init__(self, obs_shape=(4,), num_actions=2, use_lstm=False, hidden=64,
+                 use_linear_attention=False):
         nn.Module.__init__(self)
         self.obs_shape = tuple(obs_shape)
         in_dim = 1
@@ -124,7 +142,8 @@ class MLPPolicy(_CoreMixin, _HeadsMixin):
         self.fc1 = nn.Linear(in_dim, hidden)
         self.fc2 = nn.Linear(hidden, hidden)
         core_in = hidden + num_actions + 1
-        self._init_core(core_in, use_lstm)
+        self._init_core(core_in, use_lstm,
+                        use_linear_attention=use_linear_attention)
         self._init_heads(self.core_output_size, num_actions)
 
     def forward(self, inputs, core_state=(), greedy: bool = False,
@@ -148,7 +167,8 @@ class ShallowNet(_CoreMixin, _HeadsMixin):
     For 84x84 input: 84->20->9->7, flatten 32*7*7=1568.
     """
 
-    def __init__(self, obs_shape=(4, 84, 84), num_actions=6, use_lstm=False):
+    def __init__(self, obs_shape=(4, 84, 84), num_actions=6, use_lstm=False,
+                 use_linear_attention=False):
         nn.Module.__init__(self)
         self.obs_shape = tuple(obs_shape)
         c, h, w = obs_shape
@@ -163,7 +183,8 @@ class ShallowNet(_CoreMixin, _HeadsMixin):
         self.flat = 32 * h3 * w3
         self.fc = nn.Linear(self.flat, 256)
         core_in = 256 + num_actions + 1
-        self._init_core(core_in, use_lstm)
+        self._init_core(core_in, use_lstm,
+                        use_linear_attention=use_linear_attention)
         self._init_heads(self.core_output_size, num_actions)
 
     def encode(self, x: torch.Tensor) -> torch.Tensor:
@@ -236,7 +257,8 @@ class DeepResNet(_CoreMixin, _HeadsMixin):
     For 72x96 input: spatial /8 -> 9x12, flatten 32*9*12=3456 -> FC-256.
     """
 
-    def __init__(self, obs_shape=(3, 72, 96), num_actions=15, use_lstm=False):
+    def __init__(self, obs_shape=(3, 72, 96), num_actions=15, use_lstm=False,
+                 use_linear_attention=False):
         nn.Module.__init__(self)
         self.obs_shape = tuple(obs_shape)
         c, h, w = obs_shape
@@ -254,7 +276,8 @@ class DeepResNet(_CoreMixin, _HeadsMixin):
         self.flat = chans[-1] * h * w
         self.fc = nn.Linear(self.flat, 256)
         core_in = 256 + num_actions + 1
-        self._init_core(core_in, use_lstm)
+        self._init_core(core_in, use_lstm,
+                        use_linear_attention=use_linear_attention)
         self._init_heads(self.core_output_size, num_actions)
 
     def encode(self, x: torch.Tensor) -> torch.Tensor:
@@ -294,10 +317,9 @@ def build_model(flags, obs_shape, num_actions):
             kind = "deep"
         else:
             kind = "shallow"
-    if kind == "mlp":
-        return MLPPolicy(obs_shape, num_actions, use_lstm=flags.use_lstm)
-    if kind == "shallow":
-        return ShallowNet(obs_shape, num_actions, use_lstm=flags.use_lstm)
-    if kind == "deep":
-        return DeepResNet(obs_shape, num_actions, use_lstm=flags.use_lstm)
-    raise ValueError(f"unknown model {kind!r}")
+    nets = dict(mlp=MLPPolicy, shallow=ShallowNet, deep=DeepResNet)
+    if kind not in nets:
+        raise ValueError(f"unknown model {kind!r}")
+    return nets[kind](obs_shape, num_actions, use_lstm=flags.use_lstm,
+                      use_linear_attention=getattr(
+                          flags, "use_linear_attention", False))

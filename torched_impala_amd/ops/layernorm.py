@@ -81,17 +81,19 @@ class _LayerNorm(torch.autograd.Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None,
-               eps: float = 1e-5) -> torch.Tensor:
+               eps: float = 1e-5,
+               force_eager: bool = False) -> torch.Tensor:
     """Layer norm of ``x`` (..., cols) over its last axis.
 
     ``x`` is fp32, bf16 or fp16 with any strides (a copy is made only where
     its rows have no common stride or its columns are not adjacent).
     ``weight`` and ``bias`` are (cols,), fp32 or of x's type, each optional.
     Returns a contiguous tensor of x's shape and type; differentiable once
-    in x, weight and bias. Raises TypeError or ValueError for anything else.
+    in x, weight and bias. ``force_eager`` takes torch's ops instead of the
+    kernels. Raises TypeError or ValueError for anything else.
     """
     _check(x, weight, bias, eps)
-    if not (x.is_cuda and ops.hip_available()):
+    if force_eager or not (x.is_cuda and ops.hip_available()):
         # eager fallback (CPU tests / escape hatch) — same math
         f32 = torch.float32
         return torch.nn.functional.layer_norm(

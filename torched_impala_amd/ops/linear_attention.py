@@ -141,7 +141,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                      log_decay: torch.Tensor, *,
                      done: Optional[torch.Tensor] = None,
                      state: Optional[torch.Tensor] = None,
-                     scale: Optional[float] = None
+                     scale: Optional[float] = None,
+                     force_eager: bool = False
                      ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Linear attention over a time-major unroll.
 
@@ -154,7 +155,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     grow. -inf keeps nothing of the step before.
     ``done`` (T, B) bool cuts the memory before a step. ``state``
     (B, H, dk, dv) fp32 is what enters the first step, zero if left out.
-    ``scale`` defaults to dk ** -0.5.
+    ``scale`` defaults to dk ** -0.5. ``force_eager`` takes torch's ops, a
+    step at a time, instead of the kernels.
 
     Returns ``(out, final)``: out (T, B, H, dv) of q's type and the state
     behind the last step, fp32. Differentiable once in q, k, v and state,
@@ -165,7 +167,7 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """
     scale = _check("linear_attention", q, k, v, log_decay, done, state,
                    scale, 2)
-    if not (q.is_cuda and ops.hip_available()):
+    if force_eager or not (q.is_cuda and ops.hip_available()):
         return _eager(q, k, v, log_decay, done, state, scale)
     if torch.is_grad_enabled() and (
             q.requires_grad or k.requires_grad or v.requires_grad

@@ -131,7 +131,8 @@ class TrajectoryBuffers:
 
     def __init__(self, unroll_length: int, obs_shape: Tuple[int, ...],
                  obs_dtype: torch.dtype, num_actions: int, num_slots: int,
-                 lstm_hidden: int = 0, envs_per_slot: int = 1):
+                 lstm_hidden: int = 0, envs_per_slot: int = 1,
+                 core_state: Tuple[int, int] = (0, 0)):
         T = unroll_length
         n = envs_per_slot
         self.unroll_length = T
@@ -154,8 +155,11 @@ class TrajectoryBuffers:
             t = torch.zeros((num_slots, *shape), dtype=dtype)
             t.share_memory_()
             self.arenas[key] = t
-        if lstm_hidden > 0:
-            t = torch.zeros((num_slots, 2, n, lstm_hidden), dtype=torch.float32)
+        # tensors of the core's state and their size: h and c of an LSTM,
+        # or what core_state says
+        parts, size = (2, lstm_hidden) if lstm_hidden > 0 else core_state
+        if parts > 0:
+            t = torch.zeros((num_slots, parts, n, size), dtype=torch.float32)
             t.share_memory_()
             self.arenas["initial_core_state"] = t
         self._pinned = False
