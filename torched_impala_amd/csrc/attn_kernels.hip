@@ -19,11 +19,13 @@
 //   out_i = sum_j P_ij c_j + in_i a_i^T S
 //   S    <- keep S + sum_j out_j b_j c_j^T
 //
-// with in_i = e^{g(i+1)} and out_j = e^{g(L-1-j)} going forward, and the two
-// exchanged going backward; each is 0 where a done lies between. Four waves
-// split the value axis, so a wave's part of S never leaves its registers: in
-// the layout of a matrix product's result it is already the left operand of
-// the next one. Only P passes between waves, through LDS.
+// with in_i = e^{g(i+1)}, out_j = e^{g(L-1-j)} for a chunk of L rows, each 0
+// where a done lies between. Reversed roles read a chunk's rows backwards, so
+// that they run the same code; what enters them has not decayed yet and what
+// leaves has once more, in_i = e^{g i} and out_j = e^{g(L-j)}. The waves
+// split the value axis, 16 columns each, so a wave's part of S never leaves
+// its registers: in the layout of a matrix product's result it is already the
+// left operand of the next one. Only P passes between waves, through LDS.
 //
 // bf16 runs on v_mfma_f32_16x16x32_bf16. What is computed in 32 bits and has
 // to become an operand again is split into bf16 parts, so that the rounding
@@ -52,11 +54,13 @@ typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int C = 64;         // steps in a chunk: one wave's ballot of dones
-constexpr int THREADS = 256;
 
 // --------------------------------------------------------------------------
 // e^{g n}: n * log2(e) * g in two floats, so that the rounding of a long
@@ -115,29 +119,27 @@ struct EngineBF16 {
         Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
   static __device__ float at(const Frag& f, int e) { return (float)f[e]; }
-  // a fp32 value in N bf16 parts
+  // fp32 values in N bf16 parts each, two at a time as the hardware converts
   template <int N>
   static __device__ void split(const float* v, Frag* out) {
     #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float x = v[e];
+    for (int e = 0; e < 8; e += 2) {
+      f32x2 x = {v[e], v[e + 1]};
       #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const bf16_t h = (bf16_t)x;
-        out[n][e] = h;
-        x -= (float)h;
+        const bf16x2 h = __builtin_convertvector(x, bf16x2);
+        out[n][e] = h[0];
+        out[n][e + 1] = h[1];
+        if (n + 1 < N) x -= __builtin_convertvector(h, f32x2);
       }
     }
   }
-  static __device__ void store4(L* p, long part, const float* v) {
-    bf16x4 h, w;
-    #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      h[r] = (bf16_t)v[r];
-      w[r] = (bf16_t)(v[r] - (float)h[r]);
-    }
+  static __device__ void store4(L* p, int part, const float* v) {
+    const f32x4 x = {v[0], v[1], v[2], v[3]};
+    const bf16x4 h = __builtin_convertvector(x, bf16x4);
     *reinterpret_cast<bf16x4*>(p) = h;
-    *reinterpret_cast<bf16x4*>(p + part) = w;
+    *reinterpret_cast<bf16x4*>(p + part) = __builtin_convertvector(
+        x - __builtin_convertvector(h, f32x4), bf16x4);
   }
 };
 
@@ -181,7 +183,7 @@ struct EngineF32 {
     #pragma unroll
     for (int e = 0; e < 8; ++e) out[0].x[e >> 2][e & 3] = v[e];
   }
-  static __device__ void store4(L* p, long, const float* v) {
+  static __device__ void store4(L* p, int, const float* v) {
     f32x4 q = {v[0], v[1], v[2], v[3]};
     *reinterpret_cast<f32x4*>(p) = q;
   }
@@ -191,45 +193,65 @@ template <typename T> struct EngineOf { typedef EngineF32 E; };
 template <> struct EngineOf<bf16_t> { typedef EngineBF16 E; };
 
 // --------------------------------------------------------------------------
-// one chunk's rows of one operand, in registers on the way to LDS
+// One chunk's rows of one operand, in registers on the way to LDS. Loads take
+// no branch: places beyond the rows and columns are clamped to real ones and
+// cleared on the way out. (With a branch, the compiler merges its sides by
+// copies that wait for the loads on the spot.)
 // --------------------------------------------------------------------------
 template <typename T, int D, bool VEC>
 struct Rows {
+  static constexpr int THREADS = 4 * D;
   static constexpr int V = 16 / sizeof(T);
   static constexpr int PER_ROW = D / V;
-  static constexpr int N = C * PER_ROW / THREADS;
-  union Piece { uint4 q; T v[V]; };
+  static constexpr int STEP = THREADS / PER_ROW;   // rows between pieces
+  static constexpr int N = C / STEP;
+  union Piece { u32x4 q; T v[V]; };
   Piece r[N];
+  int row, col;
 
-  // rows at `p` (already at the head's first column), L of them, d columns;
-  // zeros beyond
-  __device__ void load(const T* p, long stride, int L, int d) {
+  __device__ Rows() {
+    row = threadIdx.x / PER_ROW;
+    col = (threadIdx.x % PER_ROW) * V;
+  }
+  // len rows in the order of travel, d columns, p at the lowest step's row
+  __device__ void load(const T* p, long stride, int len, int d, bool rev) {
     #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int idx = n * THREADS + threadIdx.x;
-      const int row = idx / PER_ROW, col = (idx % PER_ROW) * V;
-      r[n].q = make_uint4(0, 0, 0, 0);
-      if (row < L && col < d) {
-        const T* q = p + row * stride + col;
-        if constexpr (VEC) {
-          r[n].q = *reinterpret_cast<const uint4*>(q);
-        } else {
-          #pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (col + e < d) r[n].v[e] = q[e];
-        }
+      int i = row + n * STEP;
+      i = i < len ? i : len - 1;
+      i = rev ? len - 1 - i : i;
+      if constexpr (VEC) {   // 64 rows lie within 32 bits
+        const unsigned off = (unsigned)i * (unsigned)(stride * sizeof(T)) +
+                             (col < d ? col : 0) * (unsigned)sizeof(T);
+        r[n].q = *reinterpret_cast<const u32x4*>(
+            reinterpret_cast<const char*>(p) + off);
+      } else {
+        const T* q = p + i * stride;
+        #pragma unroll
+        for (int e = 0; e < V; ++e) r[n].v[e] = q[col + e < d ? col + e : 0];
       }
     }
   }
   template <typename LT>
-  __device__ void store(LT* s, int ld) const {
+  __device__ void store(LT* s, int ld, int len, int d) {
+    if (len < C || d < D) {
+      #pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if constexpr (VEC) {
+          if (row + n * STEP >= len || col >= d) r[n].q = u32x4{0, 0, 0, 0};
+        } else {
+          #pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (row + n * STEP >= len || col + e >= d) r[n].v[e] = (T)0.f;
+        }
+      }
+    }
+    LT* p = s + row * ld + col;
     #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const int idx = n * THREADS + threadIdx.x;
-      const int row = idx / PER_ROW, col = (idx % PER_ROW) * V;
-      LT* q = s + row * ld + col;
+      LT* q = p + n * STEP * ld;
       if constexpr (sizeof(LT) == sizeof(T)) {
-        *reinterpret_cast<uint4*>(q) = r[n].q;
+        *reinterpret_cast<u32x4*>(q) = r[n].q;
       } else {   // fp16 in fp32
         #pragma unroll
         for (int e = 0; e < V; e += 4) {
@@ -243,31 +265,45 @@ struct Rows {
   }
 };
 
+// waves that a SIMD holds: as many as the LDS of a CU leaves room for, which
+// sets how many registers a wave may take
+template <typename T, int D>
+constexpr int waves_per_simd() {
+  return sizeof(typename EngineOf<T>::E::L) == 4 ? 2
+         : D == 64 || D == 96 ? 3 : 2;
+}
+
 // --------------------------------------------------------------------------
-// T: type of the operands. D: head size as it is padded, 64 or 128.
-// VEC: 16-byte loads. STATE_ONLY: the first pass of cut sequences, which
-// leaves a segment's own state and has no rows of a result.
+// T: type of the operands. D: head size as it is padded, 32 to 128; D / 16
+// waves. VEC: 16-byte loads. STATE_ONLY: the first pass of cut sequences,
+// which leaves a segment's own state and has no rows of a result.
+//
+// Nothing inside a chunk branches on its length: rows and columns beyond the
+// real ones are zeros in LDS and cost less than the waits between the basic
+// blocks that a test of every 16 x 16 block makes (measured on one chunk of
+// fp32, 64 wide: 6 us with the tests, see below without).
 // --------------------------------------------------------------------------
 template <typename T, int D, bool VEC, bool STATE_ONLY>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(4 * D, (waves_per_simd<T, D>()))
 attn_chunks(AttnArgs args) {
   typedef typename EngineOf<T>::E E;
   typedef typename E::L L;
   typedef typename E::Frag Frag;
+  constexpr int THREADS = 4 * D;
+  constexpr int NW = D / 16;      // waves
   constexpr int LD = D + E::PAD;
   constexpr int LDP = C + E::PAD;
   constexpr int NT = D / 16;      // 16-row blocks of the state's first axis
-  constexpr int NV = D / 64;      // 16-column blocks of a wave's value axis
-  constexpr long PART = (long)C * LDP;
+  constexpr int PART = C * LDP;
 
   __shared__ __align__(16) L sa[STATE_ONLY ? 1 : C * LD];
   __shared__ __align__(16) L sb[C * LD];
   __shared__ __align__(16) L sc[C * LD];
-  __shared__ __align__(16) L sp[STATE_ONLY ? 1 : E::NP * C * LDP];
+  __shared__ __align__(16) L sp[STATE_ONLY ? 8 : E::NP * PART];
   __shared__ float pw[C + 1];
   __shared__ __align__(16) float w_out[C];
   __shared__ float w_in[C];
-  __shared__ short2 span[C];
+  __shared__ int first[C];        // first row that a row still sees
 
   const int tid = threadIdx.x;
   const int l = tid & 63, m = l & 15, g = l >> 4;
@@ -275,25 +311,23 @@ attn_chunks(AttnArgs args) {
 
   // blocks of one item (head and segment) in all roles go to one XCD, whose
   // L2 then holds the rows that the roles share
-  const long items = (long)args.B * args.H * args.nseg;
-  const int nr = args.nroles;
-  const long id = blockIdx.x;
-  const long full = items / 8 * 8;     // the last items % 8 are laid out plainly
-  long item;
-  int role_i;
+  const unsigned heads = args.B * args.H;
+  const unsigned items = heads * args.nseg;
+  const unsigned nr = args.nroles, id = blockIdx.x;
+  const unsigned full = items & ~7u;   // the last few are laid out plainly
+  unsigned item, role_i;
   if (id < full * nr) {
-    const long slot = id >> 3;
-    role_i = (int)(slot % nr);
+    const unsigned slot = id >> 3;
+    role_i = slot % nr;
     item = (slot / nr) * 8 + (id & 7);
   } else {
-    const long rest = id - full * nr;
-    role_i = (int)(rest % nr);
+    const unsigned rest = id - full * nr;
+    role_i = rest % nr;
     item = full + rest / nr;
   }
   const AttnRole& R = args.role[role_i];
-  const int seg = (int)(item / ((long)args.B * args.H));
-  const long bh = item % ((long)args.B * args.H);
-  const int b = (int)(bh / args.H), h = (int)(bh % args.H);
+  const unsigned seg = item / heads, bh = item - seg * heads;
+  const unsigned b = bh / args.H, h = bh - b * args.H;
   const int dk = R.dk, dv = R.dv;
   const bool rev = R.rev != 0;
 
@@ -305,393 +339,373 @@ attn_chunks(AttnArgs args) {
   const T* pa = (const T*)R.a.p + b * R.a.sb + h * R.a.sh;
   const T* pb = (const T*)R.b.p + b * R.b.sb + h * R.b.sh;
   const T* pc = (const T*)R.c.p + b * R.c.sb + h * R.c.sh;
-  T* po = (T*)R.out + ((long)b * args.H + h) * dv;
-  const long so = (long)args.B * args.H * dv;
-  const unsigned char* pd = args.done ? args.done + b * args.done_sb : nullptr;
+  T* po = (T*)R.out + (long)bh * dv;
+  const long so = (long)heads * dv;
+  // without flags a byte is read that is not looked at
+  const bool has_done = args.done != nullptr;
+  const unsigned char* pd =
+      has_done ? args.done + b * args.done_sb
+               : reinterpret_cast<const unsigned char*>(args.log_decay);
+  const long done_st = has_done ? args.done_st : 0;
 
-  const Decay decay(args.log_decay[h * args.g_stride]);
-  if (tid <= C) pw[tid] = decay.pow((float)tid);
-  if constexpr (!STATE_ONLY) {
-    // blocks of P that the mask leaves out and a step over 32 values of k
-    // touches stay zero
-    for (int i = tid; i < E::NP * C * LDP; i += THREADS) sp[i] = (L)0.f;
-  }
+  Rows<T, D, VEC> ra, rb, rc;
+  unsigned dn = 0;   // as loaded: a test here would wait for all loads
+  // chunk n in the order of travel: its lowest step
+  auto chunk_at = [&](int n) __attribute__((always_inline)) {
+    return t_lo + (long)(rev ? chunks - 1 - n : n) * C;
+  };
+  // behind the last chunk one row of it is read again and not used
+  auto fetch = [&](int n) __attribute__((always_inline)) {
+    const bool real = n < chunks;
+    const long t0 = chunk_at(real ? n : chunks - 1);
+    const int len = !real ? 1 : (int)(t_hi - t0 < C ? t_hi - t0 : C);
+    dn = pd[(t0 + (l < len ? l : len - 1)) * done_st];
+    if constexpr (!STATE_ONLY)
+      ra.load(pa + t0 * R.a.st, R.a.st, len, dk, rev);
+    rb.load(pb + t0 * R.b.st, R.b.st, len, dk, rev);
+    rc.load(pc + t0 * R.c.st, R.c.st, len, dv, rev);
+  };
+  fetch(0);
 
-  // the wave's part of S: block t, columns 16 (wave + 4 v) + m, rows
-  // 16 t + 4 g + r
-  f32x4 S[NT][NV];
-  const float* s_in = R.s_in;
-  bool any_state = s_in != nullptr;
+  // the wave's part of S: block t, column y, rows 16 t + 4 g + r
+  f32x4 S[NT];
+  const int y = 16 * wave + m;
+  const bool whole = dk == D && dv == D;
   const long s_size = (long)dk * dv;
+  bool any_state = R.s_in != nullptr;
   #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      S[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (any_state) {
-        const int y = 16 * (wave + 4 * v) + m;
-        const float* q = s_in + ((long)seg * args.B * args.H + bh) * s_size;
+  for (int t = 0; t < NT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (any_state) {
+    const float* q = R.s_in + ((long)seg * heads + bh) * s_size;
+    const int sx = (int)R.sx, sy = (int)R.sy;
+    if (whole) {
+      const unsigned at = 4 * g * sx + y * sy;
+      #pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) S[t][r] = (q + (16 * t + r) * sx)[at];
+      }
+    } else {   // from clamped places, all at once, and cleared beyond the size
+      q += (y < dv ? y : dv - 1) * sy;
+      #pragma unroll
+      for (int t = 0; t < NT; ++t) {
         #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int x = 16 * t + 4 * g + r;
-          if (x < dk && y < dv) S[t][v][r] = q[x * R.sx + y * R.sy];
+          S[t][r] = q[(x < dk ? x : dk - 1) * sx];
         }
+      }
+      #pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        #pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * t + 4 * g + r >= dk || y >= dv) S[t][r] = 0.f;
       }
     }
   }
 
-  Rows<T, D, VEC> ra, rb, rc;
-  int dn = 0;
-  auto chunk_at = [&](int n) {
-    return t_lo + (long)(rev ? chunks - 1 - n : n) * C;
-  };
-  auto fetch = [&](int n) {
-    const long t0 = chunk_at(n);
-    const int len = (int)(t_hi - t0 < C ? t_hi - t0 : C);
-    if constexpr (!STATE_ONLY) ra.load(pa + t0 * R.a.st, R.a.st, len, dk);
-    rb.load(pb + t0 * R.b.st, R.b.st, len, dk);
-    rc.load(pc + t0 * R.c.st, R.c.st, len, dv);
-    dn = (pd && l < len) ? pd[(t0 + l) * args.done_st] : 0;
-  };
-  fetch(0);
+  const Decay decay(args.log_decay[h * args.g_stride]);
+  for (int i = tid; i <= C; i += THREADS) pw[i] = decay.pow((float)i);
+  if constexpr (!STATE_ONLY) {
+    // blocks of P that the mask leaves out stay zero
+    u32x4* z = reinterpret_cast<u32x4*>(sp);
+    constexpr int NZ = E::NP * PART * (int)sizeof(L) / 16;
+    for (int i = tid; i < NZ; i += THREADS) z[i] = u32x4{0, 0, 0, 0};
+  }
   bool seen_done = false;
   __syncthreads();
 
-  // e^{g |i - j|} of a lane's places in a block, by the blocks' distance
-  float wt[4][4];
+  // the wave's blocks of P (ten on and under the diagonal, over the waves)
+  // and e^{g (i - j)} at the lane's places in them, 0 above the diagonal
+  constexpr int NP = (10 + NW - 1) / NW;
+  float wt[NP][4];
+  int p_it[NP], p_jt[NP];
   if constexpr (!STATE_ONLY) {
     #pragma unroll
-    for (int d = 0; d < 4; ++d) {
+    for (int e = 0; e < NP; ++e) {
+      // a wave without a block of its own computes the last one too
+      const int k = wave + NW * e < 10 ? wave + NW * e : 9;
+      p_it[e] = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0;
+      p_jt[e] = k - p_it[e] * (p_it[e] + 1) / 2;
       #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const int lag = m - 4 * g - r;
-        const int n = 16 * d + (rev ? -lag : lag);
-        wt[d][r] = pw[n < 0 ? 0 : n] * R.p_scale;
+        const int lag = 16 * (p_it[e] - p_jt[e]) + m - 4 * g - r;
+        wt[e][r] = lag < 0 ? 0.f : pw[lag > C ? C : lag] * R.p_scale;
       }
     }
   }
+  // this wave has columns of the result
+  const bool idle = 16 * wave >= dv;
 
   for (int n = 0; n < chunks; ++n) {
     const long t0 = chunk_at(n);
     const int len = (int)(t_hi - t0 < C ? t_hi - t0 : C);
-    const int nt = (len + 15) >> 4;
 
     // ---- stage: rows to LDS, weights of the chunk's rows
-    if constexpr (!STATE_ONLY) ra.store(sa, LD);
-    rb.store(sb, LD);
-    rc.store(sc, LD);
-    const unsigned long long dones = __ballot(dn != 0);
+    if constexpr (!STATE_ONLY) ra.store(sa, LD, len, dk);
+    rb.store(sb, LD, len, dk);
+    rc.store(sc, LD, len, dv);
+    // cuts between rows in the order of travel: bit i lies before row i. A
+    // done lies before its step, so backwards one row further on, and that
+    // of the lowest step behind the chunk
+    unsigned long long cuts = __ballot(has_done && dn != 0 && l < len);
+    const bool any_cut = cuts != 0;
+    bool cut_behind = false;
+    if (rev && any_cut) {
+      cut_behind = cuts & 1;
+      cuts = len > 1 ? __brevll(cuts >> 1) >> (C - len) : 0;
+    }
     if (tid < C) {
       const unsigned long long upto = (2ull << tid) - 1;   // bits 0..tid
-      const unsigned long long low = dones & upto, high = dones & ~upto;
-      const float front = low ? 0.f : pw[tid + 1];
-      const float back = (high || tid >= len) ? 0.f : pw[len - 1 - tid];
-      w_in[tid] = (rev ? back : front) * R.in_scale;
-      w_out[tid] = (rev ? (tid < len ? front : 0.f) : back) * R.u_scale;
-      span[tid] = rev
-          ? make_short2((short)tid,
-                        (short)(high ? __ffsll(high) - 2 : C - 1))
-          : make_short2((short)(low ? 63 - __clzll(low) : 0), (short)tid);
+      const unsigned long long low = cuts & upto, high = cuts & ~upto;
+      const int in = rev ? tid : tid + 1, out = rev ? len - tid : len - 1 - tid;
+      w_in[tid] = low ? 0.f : pw[in] * R.in_scale;
+      w_out[tid] = high || cut_behind || tid >= len ? 0.f
+                                                    : pw[out] * R.u_scale;
+      first[tid] = low ? 63 - __clzll(low) : 0;
     }
-    const float keep = dones ? 0.f : pw[len];
-    seen_done |= dones != 0;
+    const float keep = any_cut ? 0.f : pw[len];
+    seen_done |= any_cut;
     __syncthreads();
-    if (n + 1 < chunks) fetch(n + 1);
+    fetch(n + 1);
 
-    // columns of the value axis that this wave works on
-    const bool idle = 16 * wave >= dv;
     bool finite = true;
-
     if constexpr (!STATE_ONLY) {
       // ---- P, transposed in the products (a result's column is row i, its
-      // rows are j), ten blocks over four waves
+      // rows are j), ten blocks over the waves
+      f32x4 acc[NP];
       #pragma unroll
-      for (int e = 0; e < 3; ++e) {
-        const int k = wave + 4 * e;
-        if (k < 10) {
-          const int hi = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0;
-          const int lo = k - hi * (hi + 1) / 2;
-          const int it = rev ? lo : hi, jt = rev ? hi : lo;
-          if (hi < nt) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-            #pragma unroll
-            for (int s = 0; s < D / 32; ++s) {
-              if (32 * s < dk)
-                acc = E::mma(E::rows(sb, LD, 16 * jt, 32 * s, l),
-                             E::rows(sa, LD, 16 * it, 32 * s, l), acc);
-            }
-            const int i = 16 * it + m;
-            const short2 sp_i = span[i];
-            float p[4];
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int j = 16 * jt + 4 * g + r;
-              const int d = hi - lo;
-              const float w = d == 0 ? wt[0][r] : d == 1 ? wt[1][r]
-                              : d == 2 ? wt[2][r] : wt[3][r];
-              p[r] = (j >= sp_i.x && j <= sp_i.y) ? acc[r] * w : 0.f;
-            }
-            E::store4(sp + i * LDP + 16 * jt + 4 * g, PART, p);
-          }
+      for (int e = 0; e < NP; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+      #pragma unroll
+      for (int s = 0; s < D / 32; ++s) {
+        #pragma unroll
+        for (int e = 0; e < NP; ++e)
+          acc[e] = E::mma(E::rows(sb, LD, 16 * p_jt[e], 32 * s, l),
+                          E::rows(sa, LD, 16 * p_it[e], 32 * s, l), acc[e]);
+      }
+      float p[NP][4];
+      #pragma unroll
+      for (int e = 0; e < NP; ++e) {
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) p[e][r] = acc[e][r] * wt[e][r];
+      }
+      if (any_cut) {
+        #pragma unroll
+        for (int e = 0; e < NP; ++e) {
+          const int lo = first[16 * p_it[e] + m] - 16 * p_jt[e] - 4 * g;
+          #pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (r < lo) p[e][r] = 0.f;
         }
       }
-      __syncthreads();
+      #pragma unroll
+      for (int e = 0; e < NP; ++e)
+        E::store4(sp + (16 * p_it[e] + m) * LDP + 16 * p_jt[e] + 4 * g, PART,
+                  p[e]);
     }
 
-    f32x4 O[NV][4];
-    Frag cf[2][NV];
+    f32x4 O[4];
+    Frag cf[2];
     if (!idle) {
       if constexpr (!STATE_ONLY) {
         // ---- what came before the chunk: a S, weighted per row
         #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-          #pragma unroll
-          for (int it = 0; it < 4; ++it) O[v][it] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
+        for (int it = 0; it < 4; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (any_state) {
           #pragma unroll
           for (int s = 0; s < D / 32; ++s) {
-            if (32 * s < dk) {
-              Frag sf[NV][E::NP];
+            Frag sf[E::NP];
+            float x[8];
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              x[r] = S[2 * s][r];
+              x[4 + r] = S[2 * s + 1][r];
+            }
+            E::template split<E::NP>(x, sf);
+            #pragma unroll
+            for (int it = 0; it < 4; ++it) {
+              const Frag af = E::rows(sa, LD, 16 * it, 32 * s, l);
               #pragma unroll
-              for (int v = 0; v < NV; ++v) {
-                float x[8];
-                #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                  x[r] = S[2 * s][v][r];
-                  x[4 + r] = S[2 * s + 1][v][r];
-                }
-                E::template split<E::NP>(x, sf[v]);
-              }
-              #pragma unroll
-              for (int it = 0; it < 4; ++it) {
-                if (it < nt) {
-                  const Frag af = E::rows(sa, LD, 16 * it, 32 * s, l);
-                  #pragma unroll
-                  for (int v = 0; v < NV; ++v) {
-                    #pragma unroll
-                    for (int p = 0; p < E::NP; ++p)
-                      O[v][it] = E::mma(sf[v][p], af, O[v][it]);
-                  }
-                }
-              }
+              for (int p = 0; p < E::NP; ++p)
+                O[it] = E::mma(sf[p], af, O[it]);
             }
           }
           #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const float w = w_in[16 * it + m];
             #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-              #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                O[v][it][r] = w == 0.f ? 0.f : O[v][it][r] * w;
-            }
+            for (int r = 0; r < 4; ++r)
+              O[it][r] *= w;
           }
         }
       }
       // ---- c, as it is needed twice: left operand here, right one below
       #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        #pragma unroll
-        for (int v = 0; v < NV; ++v)
-          cf[s][v] = E::cols(sc, LD, 32 * s, 16 * (wave + 4 * v), l);
-      }
+      for (int s = 0; s < 2; ++s)
+        cf[s] = E::cols(sc, LD, 32 * s, 16 * wave, l);
+    }
+    if constexpr (!STATE_ONLY) __syncthreads();   // P is whole
+    if (!idle) {
       if constexpr (!STATE_ONLY) {
+        // row blocks 0 and 1 meet the first 32 rows of j, 2 and 3 all
         #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          if (it < nt) {
+          #pragma unroll
+          for (int s = 0; s <= it >> 1; ++s) {
             #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              // rows 32 s .. 32 s + 31 of j meet row block `it`?
-              if (rev ? 2 * s + 1 >= it : 2 * s <= it) {
-                #pragma unroll
-                for (int p = 0; p < E::NP; ++p) {
-                  const Frag pf =
-                      E::rows(sp + p * PART, LDP, 16 * it, 32 * s, l);
-                  #pragma unroll
-                  for (int v = 0; v < NV; ++v)
-                    O[v][it] = E::mma(cf[s][v], pf, O[v][it]);
-                }
-              }
-            }
+            for (int p = 0; p < E::NP; ++p)
+              O[it] = E::mma(cf[s],
+                             E::rows(sp + p * PART, LDP, 16 * it, 32 * s, l),
+                             O[it]);
           }
         }
-        float z = 0.f;
+        // An input that is not finite always shows in the row that it
+        // belongs to, where its own weight is not zero; a state that is not
+        // shows in every row, as weights of zero make NaN of it.
+        f32x4 z = {0.f, 0.f, 0.f, 0.f};
         #pragma unroll
-        for (int v = 0; v < NV; ++v) {
+        for (int it = 0; it < 4; ++it) {
           #pragma unroll
-          for (int it = 0; it < 4; ++it) {
-            #pragma unroll
-            for (int r = 0; r < 4; ++r) z = fmaf(O[v][it][r], 0.f, z);
-          }
+          for (int r = 0; r < 4; ++r) z[r] = fmaf(O[it][r], 0.f, z[r]);
         }
-        // an input that is not finite always shows in the row that it
-        // belongs to, where its own weight is not masked
-        finite = !__any(z != 0.f);
+        finite = !__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f);
         if (finite) {
-          #pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            const int y = 16 * (wave + 4 * v) + 4 * g;
+          const int x0 = 16 * wave + 4 * g;
+          if constexpr (VEC) {   // dv is a multiple of 4, 64 rows in 32 bits
+            T* q = po + (rev ? t0 + len - C : t0) * so;
+            const long step = (rev ? -16 : 16) * so;
+            const unsigned at = (unsigned)((rev ? C - 1 - m : m) * so + x0);
+            #pragma unroll
+            for (int it = 0; it < 4; ++it) {
+              struct alignas(4 * sizeof(T)) { T e[4]; } w;
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) w.e[r] = (T)O[it][r];
+              if (16 * it + m < len && x0 < dv)
+                *reinterpret_cast<decltype(w)*>(q + it * step + at) = w;
+            }
+          } else {
             #pragma unroll
             for (int it = 0; it < 4; ++it) {
               const int i = 16 * it + m;
-              if (i < len && y < dv) {
-                T* q = po + (t0 + i) * so + y;
-                if ((dv & 3) == 0) {
-                  struct alignas(4 * sizeof(T)) { T e[4]; } w;
-                  #pragma unroll
-                  for (int r = 0; r < 4; ++r) w.e[r] = (T)O[v][it][r];
-                  *reinterpret_cast<decltype(w)*>(q) = w;
-                } else {
-                  #pragma unroll
-                  for (int r = 0; r < 4; ++r)
-                    if (y + r < dv) q[r] = (T)O[v][it][r];
-                }
-              }
+              T* q = po + (t0 + (rev ? len - 1 - i : i)) * so + x0;
+              #pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (i < len && x0 + r < dv) q[r] = (T)O[it][r];
             }
           }
         }
       }
       // ---- the state behind the chunk
-      f32x4 U[STATE_ONLY ? NT : 1][STATE_ONLY ? NV : 1];
       if (finite) {
-        Frag cw[2][NV][E::NU];
+        Frag cw[2][E::NU];
         #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const f32x4 w0 = *reinterpret_cast<const f32x4*>(
               w_out + 32 * s + 4 * g);
           const f32x4 w1 = *reinterpret_cast<const f32x4*>(
               w_out + 32 * s + 16 + 4 * g);
+          float x[8];
           #pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            float x[8];
-            #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float w = e < 4 ? w0[e & 3] : w1[e & 3];
-              x[e] = w == 0.f ? 0.f : E::at(cf[s][v], e) * w;
-            }
-            E::template split<E::NU>(x, cw[s][v]);
+          for (int e = 0; e < 8; ++e) {
+            x[e] = E::at(cf[s], e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
           }
+          E::template split<E::NU>(x, cw[s]);
         }
+        f32x4 U[NT];
         #pragma unroll
         for (int t = 0; t < NT; ++t) {
-          if (16 * t < dk) {
-            f32x4 acc[NV];
+          #pragma unroll
+          for (int r = 0; r < 4; ++r) U[t][r] = S[t][r] * keep;
+        }
+        #pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          #pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const Frag bf = E::cols(sb, LD, 32 * s, 16 * t, l);
             #pragma unroll
-            for (int v = 0; v < NV; ++v) acc[v] = f32x4{0.f, 0.f, 0.f, 0.f};
-            #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-              if (32 * s < len) {
-                const Frag bf = E::cols(sb, LD, 32 * s, 16 * t, l);
-                #pragma unroll
-                for (int v = 0; v < NV; ++v) {
-                  #pragma unroll
-                  for (int p = 0; p < E::NU; ++p)
-                    acc[v] = E::mma(bf, cw[s][v][p], acc[v]);
-                }
-              }
-            }
-            #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-              if constexpr (STATE_ONLY) {
-                U[t][v] = acc[v];
-              } else {
-                #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  S[t][v][r] = (keep == 0.f ? 0.f : S[t][v][r] * keep) +
-                               acc[v][r];
-              }
-            }
-          } else if constexpr (STATE_ONLY) {
-            #pragma unroll
-            for (int v = 0; v < NV; ++v) U[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int p = 0; p < E::NU; ++p) U[t] = E::mma(bf, cw[s][p], U[t]);
           }
         }
-        if constexpr (STATE_ONLY) {
-          float z = 0.f;
+        if constexpr (STATE_ONLY) {   // no rows that would show it
+          f32x4 z = {0.f, 0.f, 0.f, 0.f};
           #pragma unroll
           for (int t = 0; t < NT; ++t) {
             #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-              #pragma unroll
-              for (int r = 0; r < 4; ++r) z = fmaf(U[t][v][r], 0.f, z);
-            }
+            for (int r = 0; r < 4; ++r) z[r] = fmaf(U[t][r], 0.f, z[r]);
           }
-          finite = !__any(z != 0.f);
-          if (finite) {
-            #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              #pragma unroll
-              for (int v = 0; v < NV; ++v) {
-                #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  S[t][v][r] = (keep == 0.f ? 0.f : S[t][v][r] * keep) +
-                               U[t][v][r];
-              }
-            }
-          }
+          finite = !__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f);
+        }
+        if (finite) {
+          #pragma unroll
+          for (int t = 0; t < NT; ++t) S[t] = U[t];
         }
       }
       // ---- step by step, where something is not finite
       if (!finite) {
-        for (int q = 0; q < len; ++q) {
-          const int i = rev ? len - 1 - q : q;
-          const bool cut = (dones >> i) & 1;
-          float o[NV];
+        for (int i = 0; i < len; ++i) {
+          // what lies before the first row backwards has not decayed
+          const bool cut = (cuts >> i) & 1;
+          const float f = rev && i == 0 ? 1.f : pw[1];
+          const float cy = (float)sc[i * LD + y] * R.u_scale;
+          float o = 0.f;
           #pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            o[v] = 0.f;
-            const int y = 16 * (wave + 4 * v) + m;
-            const float cy = (float)sc[i * LD + y] * R.u_scale;
+          for (int t = 0; t < NT; ++t) {
             #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              #pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const int x = 16 * t + 4 * g + r;
-                if (x < dk && y < dv) {
-                  float s = S[t][v][r];
-                  if (!rev) s = cut ? 0.f : s * pw[1];
-                  s = fmaf((float)sb[i * LD + x], cy, s);
-                  if constexpr (!STATE_ONLY)
-                    o[v] = fmaf((float)sa[i * LD + x], s, o[v]);
-                  if (rev) s = cut ? 0.f : s * pw[1];
-                  S[t][v][r] = s;
-                }
+            for (int r = 0; r < 4; ++r) {
+              const int x = 16 * t + 4 * g + r;
+              if (x < dk && y < dv) {
+                S[t][r] = fmaf((float)sb[i * LD + x], cy,
+                               cut ? 0.f : S[t][r] * f);
+                if constexpr (!STATE_ONLY)
+                  o = fmaf((float)sa[i * LD + x], S[t][r], o);
               }
             }
-            if constexpr (!STATE_ONLY) {
-              o[v] += __shfl_xor(o[v], 16, 64);
-              o[v] += __shfl_xor(o[v], 32, 64);
-              if (g == 0 && y < dv)
-                po[(t0 + i) * so + y] = (T)(o[v] * R.in_scale);
-            }
+          }
+          if constexpr (!STATE_ONLY) {
+            o += __shfl_xor(o, 16, 64);
+            o += __shfl_xor(o, 32, 64);
+            if (g == 0 && y < dv)
+              po[(t0 + (rev ? len - 1 - i : i)) * so + y] =
+                  (T)(o * R.in_scale);
+          }
+        }
+        if (rev) {
+          #pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            #pragma unroll
+            for (int r = 0; r < 4; ++r)
+              S[t][r] = cut_behind ? 0.f : S[t][r] * pw[1];
           }
         }
       }
     }
     any_state = true;
-    __syncthreads();   // LDS is free for the next chunk
+    if (n + 1 < chunks) __syncthreads();   // LDS is free for the next chunk
   }
 
   if (STATE_ONLY && tid == 0)
-    args.keep[(long)seg * args.B * args.H + bh] =
+    args.keep[seg * heads + bh] =
         seen_done ? 0.f : decay.pow((float)(t_hi - t_lo));
 
   // the state behind the last step of this pass: a segment's own in the
   // first pass, the whole sequence's in the main one
-  float* s_out = R.s_out;
-  if (STATE_ONLY || (s_out && seg == (rev ? 0 : args.nseg - 1))) {
-    float* q = s_out +
-               (STATE_ONLY ? (long)seg * args.B * args.H + bh : bh) * s_size;
-    #pragma unroll
-    for (int t = 0; t < NT; ++t) {
+  if (STATE_ONLY || (R.s_out && (int)seg == (rev ? 0 : args.nseg - 1))) {
+    float* q = R.s_out + (STATE_ONLY ? (long)seg * heads + bh : (long)bh) *
+                             s_size;
+    if (whole) {
+      const unsigned at = 4 * g * D + y;
       #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int y = 16 * (wave + 4 * v) + m;
+      for (int t = 0; t < NT; ++t) {
+        #pragma unroll
+        for (int r = 0; r < 4; ++r) (q + (16 * t + r) * D)[at] = S[t][r];
+      }
+    } else {
+      #pragma unroll
+      for (int t = 0; t < NT; ++t) {
         #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int x = 16 * t + 4 * g + r;
-          if (x < dk && y < dv) q[(long)x * dv + y] = S[t][v][r];
+          if (x < dk && y < dv) q[x * dv + y] = S[t][r];
         }
       }
     }
@@ -812,29 +826,32 @@ attn_step(AttnStepArgs A) {
 
 template <typename T, int D, bool VEC>
 void run(const AttnArgs& a, bool state_only, hipStream_t s) {
-  const long items = (long)a.B * a.H * a.nseg * a.nroles;
+  const dim3 grid((unsigned)((long)a.B * a.H * a.nseg * a.nroles));
   if (state_only)
-    hipLaunchKernelGGL((attn_chunks<T, D, VEC, true>), dim3((unsigned)items),
-                       dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL((attn_chunks<T, D, VEC, true>), grid, dim3(4 * D), 0,
+                       s, a);
   else
-    hipLaunchKernelGGL((attn_chunks<T, D, VEC, false>), dim3((unsigned)items),
-                       dim3(THREADS), 0, s, a);
+    hipLaunchKernelGGL((attn_chunks<T, D, VEC, false>), grid, dim3(4 * D), 0,
+                       s, a);
 }
 
-template <typename T>
-void run_t(const AttnArgs& a, int vec, bool state_only, hipStream_t s) {
+template <typename T, bool VEC>
+void run_t(const AttnArgs& a, bool state_only, hipStream_t s) {
   int d = 0;
   for (int i = 0; i < a.nroles; ++i) {
     d = a.role[i].dk > d ? a.role[i].dk : d;
     d = a.role[i].dv > d ? a.role[i].dv : d;
   }
-  if (d <= 64) {
-    if (vec) run<T, 64, true>(a, state_only, s);
-    else run<T, 64, false>(a, state_only, s);
-  } else {
-    if (vec) run<T, 128, true>(a, state_only, s);
-    else run<T, 128, false>(a, state_only, s);
-  }
+  if (d <= 32) run<T, 32, VEC>(a, state_only, s);
+  else if (d <= 64) run<T, 64, VEC>(a, state_only, s);
+  else if (d <= 96) run<T, 96, VEC>(a, state_only, s);
+  else run<T, 128, VEC>(a, state_only, s);
+}
+
+template <typename T>
+void run_v(const AttnArgs& a, int vec, bool state_only, hipStream_t s) {
+  if (vec) run_t<T, true>(a, state_only, s);
+  else run_t<T, false>(a, state_only, s);
 }
 
 }  // namespace attn
@@ -846,9 +863,9 @@ extern "C" {
 
 void launch_attn_chunks(int type, const AttnArgs* a, int vec, int state_only,
                         hipStream_t s) {
-  if (type == 0) run_t<float>(*a, vec, state_only != 0, s);
-  else if (type == 1) run_t<bf16_t>(*a, vec, state_only != 0, s);
-  else run_t<f16_t>(*a, vec, state_only != 0, s);
+  if (type == 0) run_v<float>(*a, vec, state_only != 0, s);
+  else if (type == 1) run_v<bf16_t>(*a, vec, state_only != 0, s);
+  else run_v<f16_t>(*a, vec, state_only != 0, s);
 }
 
 void launch_attn_scan(float* st, const float* keep, const float* first,

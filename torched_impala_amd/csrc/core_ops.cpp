@@ -10,6 +10,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <vector>
 
@@ -228,9 +229,12 @@ AttnOperand operand(const Tensor& t, int lead) {
                      st(lead)};
 }
 
-// 16-byte loads: base, strides and row length are multiples of 16 bytes
+// 16-byte loads: base, strides and row length are multiples of 16 bytes, and
+// 64 steps lie within 32 bits of offsets
 bool can_vec(const Tensor& t, const AttnOperand& o) {
   const long es = t.element_size();
+  const long dense = t.size(1) * t.size(2) * t.size(-1);   // of a result
+  if (64 * es * std::max(std::abs(o.st), dense) >= (1L << 31)) return false;
   return ((uintptr_t)o.p & 15) == 0 && (o.st * es) % 16 == 0 &&
          (o.sb * es) % 16 == 0 && (o.sh * es) % 16 == 0 &&
          (t.size(-1) * es) % 16 == 0;
