@@ -7,11 +7,15 @@
 
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <memory>
+#include <tuple>
 #include <vector>
 
 #include "attn_kernels.h"
@@ -42,6 +46,8 @@ namespace {
 
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 void check_launch(const char* what) {
   const hipError_t e = hipGetLastError();
@@ -62,97 +68,161 @@ int type_code(const Tensor& t, const char* name) {
   }
 }
 
-const void* ptr(const OptTensor& t) {
-  return t.has_value() ? t->data_ptr() : nullptr;
+Tensor or_undefined(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+
+const void* ptr(const Tensor& t) {
+  return t.defined() ? t.data_ptr() : nullptr;
+}
+
+bool wants_grad(std::initializer_list<Tensor> ts) {
+  if (!torch::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// gradients of operators that are differentiable once: a second
+// differentiation raises instead of taking them for constants
+variable_list once(variable_list grads, const char* what) {
+  if (!torch::GradMode::is_enabled()) return grads;
+  variable_list in;
+  for (const Tensor& t : grads)
+    if (t.defined()) in.push_back(t.detach().requires_grad_());
+  auto stop = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " is differentiable once", (int64_t)in.size());
+  const variable_list out = (*stop)(variable_list(in));
+  size_t k = 0;
+  for (Tensor& t : grads)
+    if (t.defined()) t = out[k++];
+  return grads;
 }
 
 // ---------------------------------------------------------------------------
-// layer norm. x (rows, cols) with unit column stride; the row stride is free
+// layer norm
 // ---------------------------------------------------------------------------
-void check_norm_operands(const Tensor& x, const OptTensor& w,
-                         const OptTensor& b) {
-  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0 &&
-                  (x.stride(1) == 1 || x.size(1) == 1) && x.stride(0) >= 0,
-              "layer_norm: x must be a GPU matrix with unit column stride");
-  for (const auto* p : {&w, &b}) {
-    if (!p->has_value()) continue;
-    const Tensor& t = **p;
-    TORCH_CHECK(t.device() == x.device() && t.dim() == 1 &&
-                    t.size(0) == x.size(1) && t.is_contiguous(),
-                "layer_norm: weight and bias must be (cols,) on x's device");
-    TORCH_CHECK(t.scalar_type() == torch::kFloat32 ||
-                    t.scalar_type() == x.scalar_type(),
-                "layer_norm: weight and bias must be fp32 or of x's type");
+void check_norm(const Tensor& x, const Tensor& w, const Tensor& b,
+                double eps) {
+  TORCH_CHECK_TYPE(x.scalar_type() == torch::kFloat32 ||
+                       x.scalar_type() == torch::kBFloat16 ||
+                       x.scalar_type() == torch::kFloat16,
+                   "layer_norm: x must be fp32, bf16 or fp16, not ",
+                   x.scalar_type());
+  TORCH_CHECK_VALUE(x.is_cuda() && x.dim() >= 1 && x.size(-1) >= 1,
+                    "layer_norm: x needs a last axis of one or more");
+  for (const Tensor* t : {&w, &b}) {
+    if (!t->defined()) continue;
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == x.size(-1) &&
+                          t->device() == x.device(),
+                      "layer_norm: weight and bias must be (", x.size(-1),
+                      ",) on x's device");
+    TORCH_CHECK_TYPE(t->scalar_type() == torch::kFloat32 ||
+                         t->scalar_type() == x.scalar_type(),
+                     "layer_norm: weight and bias must be fp32 or of x's "
+                     "type");
   }
-  TORCH_CHECK(!w.has_value() || !b.has_value() ||
-                  w->scalar_type() == b->scalar_type(),
-              "layer_norm: weight and bias must have one type");
+  TORCH_CHECK_TYPE(!w.defined() || !b.defined() ||
+                       w.scalar_type() == b.scalar_type(),
+                   "layer_norm: weight and bias must have one type");
+  TORCH_CHECK_VALUE(std::isfinite(eps) && eps >= 0.0,
+                    "layer_norm: eps must be finite and >= 0, not ", eps);
 }
 
-std::vector<Tensor> layer_norm_fwd(Tensor x, OptTensor w, OptTensor b,
-                                   double eps, bool save) {
-  check_norm_operands(x, w, b);
-  const int xt = type_code(x, "x");
-  const int wt = w.has_value() ? type_code(*w, "weight")
-                 : b.has_value() ? type_code(*b, "bias") : xt;
-  const long rows = x.size(0), cols = x.size(1);
+// (rows, cols) with unit column stride: a view where strides allow
+Tensor norm_rows(const Tensor& x) {
+  Tensor r = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  return r.size(1) > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+}
+
+Tensor dense(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+// y and, if `save`, the rows' mean and rstd
+Tensor norm_fwd(const Tensor& x, const Tensor& w, const Tensor& b, double eps,
+                bool save, Tensor* stats) {
   const c10::DeviceGuard guard(x.device());
-  auto y = torch::empty({rows, cols}, x.options());
-  auto fopts = x.options().dtype(torch::kFloat32);
-  auto stats = torch::empty({2, save ? rows : 0}, fopts);
+  const Tensor xr = norm_rows(x), wc = dense(w), bc = dense(b);
+  const int xt = type_code(x, "x");
+  const int wt = w.defined() ? type_code(w, "weight")
+                 : b.defined() ? type_code(b, "bias") : xt;
+  const long rows = xr.size(0), cols = xr.size(1);
+  Tensor y = torch::empty(x.sizes(), x.options());
+  float* mean = nullptr;
+  if (save) {
+    *stats = torch::empty({2, rows}, x.options().dtype(torch::kFloat32));
+    mean = stats->data_ptr<float>();
+  }
   if (rows > 0) {
-    float* mean = save ? stats.data_ptr<float>() : nullptr;
-    launch_layer_norm_fwd(xt, wt, x.data_ptr(), x.stride(0), ptr(w), ptr(b),
-                          y.data_ptr(), mean, save ? mean + rows : nullptr,
-                          rows, cols, (float)eps, stream_here());
+    launch_layer_norm_fwd(xt, wt, xr.data_ptr(), xr.stride(0), ptr(wc),
+                          ptr(bc), y.data_ptr(), mean,
+                          save ? mean + rows : nullptr, rows, cols,
+                          (float)eps, stream_here());
     check_launch("layer_norm");
   }
-  return {y, stats};
+  return y;
 }
 
-std::vector<OptTensor> layer_norm_bwd(Tensor dy, Tensor x, OptTensor w,
-                                      Tensor stats, bool need_dx,
-                                      bool need_dw, bool need_db,
-                                      bool param_fp32) {
-  check_norm_operands(x, w, c10::nullopt);
-  const long rows = x.size(0), cols = x.size(1);
-  TORCH_CHECK(dy.device() == x.device() && dy.sizes() == x.sizes() &&
-                  dy.scalar_type() == x.scalar_type() && dy.is_contiguous(),
-              "layer_norm: the output's gradient must match the output");
-  TORCH_CHECK(stats.device() == x.device() && stats.is_contiguous() &&
-                  stats.scalar_type() == torch::kFloat32 &&
-                  stats.numel() == 2 * rows,
-              "layer_norm: saved statistics do not match x");
-  const int xt = type_code(x, "x");
-  const int wt = w.has_value() ? type_code(*w, "weight")
-                 : param_fp32 ? 0 : xt;
-  const c10::DeviceGuard guard(x.device());
-  auto popts = x.options();
-  if (wt == 0) popts = popts.dtype(torch::kFloat32);
-  OptTensor dx, dw, db;
-  if (need_dx) dx = torch::empty({rows, cols}, x.options());
-  if (rows == 0) {
-    if (need_dw) dw = torch::zeros({cols}, popts);
-    if (need_db) db = torch::zeros({cols}, popts);
-    return {dx, dw, db};
+class LayerNorm : public torch::autograd::Function<LayerNorm> {
+ public:
+  static Tensor forward(AutogradContext* ctx, Tensor x, OptTensor weight,
+                        OptTensor bias, double eps) {
+    const Tensor w = or_undefined(weight), b = or_undefined(bias);
+    Tensor stats;
+    Tensor y = norm_fwd(x, w, b, eps, true, &stats);
+    // x itself, not its 2-D view, so that a change of it in place is caught
+    ctx->save_for_backward({x, w, stats});
+    ctx->saved_data["dx"] = x.requires_grad();
+    ctx->saved_data["dw"] = w.defined() && w.requires_grad();
+    ctx->saved_data["db"] = b.defined() && b.requires_grad();
+    ctx->saved_data["type"] =
+        (int64_t)(w.defined() ? w : b.defined() ? b : x).scalar_type();
+    return y;
   }
-  if (need_dw) dw = torch::empty({cols}, popts);
-  if (need_db) db = torch::empty({cols}, popts);
-  const int al = layer_norm_aligned(xt, dy.data_ptr(), x.data_ptr(),
-                                    x.stride(0), ptr(w), ptr(dx), cols);
-  Tensor part;
-  if (need_dw || need_db)
-    part = torch::empty({layer_norm_part_elems(xt, rows, cols, al)},
-                        x.options().dtype(torch::kFloat32));
-  launch_layer_norm_bwd(
-      xt, wt, al, dy.data_ptr(), x.data_ptr(), x.stride(0), ptr(w),
-      stats.data_ptr<float>(), stats.data_ptr<float>() + rows,
-      const_cast<void*>(ptr(dx)),
-      part.defined() ? part.data_ptr<float>() : nullptr,
-      const_cast<void*>(ptr(dw)), const_cast<void*>(ptr(db)), rows, cols,
-      stream_here());
-  check_launch("layer_norm backward");
-  return {dx, dw, db};
+
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &w = saved[1], &stats = saved[2];
+    const bool need_dx = ctx->saved_data["dx"].toBool();
+    const bool need_dw = ctx->saved_data["dw"].toBool();
+    const bool need_db = ctx->saved_data["db"].toBool();
+    const auto ptype = (torch::ScalarType)ctx->saved_data["type"].toInt();
+    const c10::DeviceGuard guard(x.device());
+    const Tensor xr = norm_rows(x), wc = dense(w);
+    const Tensor dy = g[0].contiguous();
+    const long rows = xr.size(0), cols = xr.size(1);
+    const int xt = type_code(x, "x");
+    const int wt = ptype == torch::kFloat32 ? 0 : xt;
+    const auto popts = x.options().dtype(ptype);
+    Tensor dx, dw, db;
+    if (need_dx) dx = torch::empty(x.sizes(), x.options());
+    if (need_dw) dw = rows ? torch::empty({cols}, popts)
+                           : torch::zeros({cols}, popts);
+    if (need_db) db = rows ? torch::empty({cols}, popts)
+                           : torch::zeros({cols}, popts);
+    if (rows > 0) {
+      const int al = layer_norm_aligned(xt, dy.data_ptr(), xr.data_ptr(),
+                                        xr.stride(0), ptr(wc), ptr(dx), cols);
+      Tensor part;
+      if (need_dw || need_db)
+        part = torch::empty({layer_norm_part_elems(xt, rows, cols, al)},
+                            x.options().dtype(torch::kFloat32));
+      launch_layer_norm_bwd(
+          xt, wt, al, dy.data_ptr(), xr.data_ptr(), xr.stride(0), ptr(wc),
+          stats.data_ptr<float>(), stats.data_ptr<float>() + rows,
+          const_cast<void*>(ptr(dx)),
+          part.defined() ? part.data_ptr<float>() : nullptr,
+          const_cast<void*>(ptr(dw)), const_cast<void*>(ptr(db)), rows, cols,
+          stream_here());
+      check_launch("layer_norm backward");
+    }
+    return once({dx, dw, db, Tensor()}, "layer_norm");
+  }
+};
+
+Tensor layer_norm(Tensor x, OptTensor weight, OptTensor bias, double eps) {
+  const Tensor w = or_undefined(weight), b = or_undefined(bias);
+  check_norm(x, w, b, eps);
+  if (wants_grad({x, w, b}))
+    return LayerNorm::apply(x, weight, bias, eps);
+  return norm_fwd(x, w, b, eps, false, nullptr);
 }
 
 // ---------------------------------------------------------------------------
@@ -171,55 +241,74 @@ struct AttnShape {
   long T, B, H, dk, dv;
 };
 
-void check_unit(const Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), "linear_attention: ", name, " must be on GPU");
-  TORCH_CHECK(t.stride(-1) == 1 || t.size(-1) == 1,
-              "linear_attention: the last axis of ", name,
-              " must be contiguous");
+// a head's features side by side; every other stride is free
+Tensor unit(const Tensor& t) {
+  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
-AttnShape check_attn(const Tensor& q, const Tensor& k, const Tensor& v,
-                     const Tensor& g, const OptTensor& done, int lead) {
-  check_unit(q, "q");
-  check_unit(k, "k");
-  check_unit(v, "v");
-  TORCH_CHECK(q.dim() == lead + 2 && k.sizes() == q.sizes() &&
-                  v.dim() == q.dim() &&
-                  v.sizes().slice(0, lead + 1) == q.sizes().slice(0, lead + 1),
-              "linear_attention: shapes of q, k and v do not fit");
-  TORCH_CHECK(k.scalar_type() == q.scalar_type() &&
-                  v.scalar_type() == q.scalar_type() &&
-                  k.device() == q.device() && v.device() == q.device(),
-              "linear_attention: q, k and v must have one type and device");
-  AttnShape s{lead == 2 ? q.size(0) : 1, q.size(lead - 1), q.size(lead),
-              q.size(-1), v.size(-1)};
-  TORCH_CHECK(s.dk >= 1 && s.dk <= MAX_HEAD && s.dv >= 1 && s.dv <= MAX_HEAD,
-              "linear_attention: head sizes must be 1 to ", MAX_HEAD);
-  TORCH_CHECK(s.B <= MAX_GRID && s.H <= MAX_GRID,
-              "linear_attention: batch too large");
-  TORCH_CHECK(g.device() == q.device() && g.dim() == 1 &&
-                  g.size(0) == s.H && g.scalar_type() == torch::kFloat32,
-              "linear_attention: log_decay must be (H,) fp32 on q's device");
-  if (done.has_value())
-    TORCH_CHECK(done->device() == q.device() &&
-                    done->scalar_type() == torch::kBool &&
-                    done->sizes() == q.sizes().slice(0, lead),
-                "linear_attention: done must be bool, one flag a step and "
-                "environment, on q's device");
+AttnShape check_attn(const char* op, const Tensor& q, const Tensor& k,
+                     const Tensor& v, const Tensor& g, const Tensor& done,
+                     const Tensor& state, int lead) {
+  TORCH_CHECK_TYPE(q.scalar_type() == torch::kFloat32 ||
+                       q.scalar_type() == torch::kBFloat16 ||
+                       q.scalar_type() == torch::kFloat16,
+                   op, ": q must be fp32, bf16 or fp16, not ",
+                   q.scalar_type());
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() &&
+                       v.scalar_type() == q.scalar_type(),
+                   op, ": q, k and v must have one type");
+  TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() &&
+                        v.device() == q.device(),
+                    op, ": q, k and v must be on one device");
+  TORCH_CHECK_VALUE(q.dim() == lead + 2, op, ": q must have ", lead + 2,
+                    " axes, not ", q.dim());
+  TORCH_CHECK_VALUE(k.sizes() == q.sizes(), op, ": k is ", k.sizes(), ", q ",
+                    q.sizes());
+  TORCH_CHECK_VALUE(
+      v.dim() == q.dim() &&
+          v.sizes().slice(0, lead + 1) == q.sizes().slice(0, lead + 1),
+      op, ": v is ", v.sizes(), ", q ", q.sizes());
+  const AttnShape s{lead == 2 ? q.size(0) : 1, q.size(lead - 1),
+                    q.size(lead), q.size(-1), v.size(-1)};
+  TORCH_CHECK_VALUE(
+      s.dk >= 1 && s.dk <= MAX_HEAD && s.dv >= 1 && s.dv <= MAX_HEAD, op,
+      ": head sizes must be 1 to ", MAX_HEAD, ", not ", s.dk, " and ", s.dv);
+  TORCH_CHECK_VALUE(s.B <= MAX_GRID && s.H <= MAX_GRID &&
+                        s.B * s.H <= MAX_GRID / 3,
+                    op, ": batch too large");
+  TORCH_CHECK_TYPE(g.scalar_type() == torch::kFloat32, op,
+                   ": log_decay must be fp32, not ", g.scalar_type());
+  TORCH_CHECK_VALUE(g.device() == q.device() && g.dim() == 1 &&
+                        g.size(0) == s.H,
+                    op, ": log_decay must be (", s.H, ",) on q's device");
+  TORCH_CHECK_VALUE(!g.requires_grad(), op,
+                    ": log_decay is a head's fixed slope and gets no "
+                    "gradient; pass it detached");
+  if (done.defined()) {
+    TORCH_CHECK_TYPE(done.scalar_type() == torch::kBool, op,
+                     ": done must be bool, not ", done.scalar_type());
+    TORCH_CHECK_VALUE(done.device() == q.device() &&
+                          done.sizes() == q.sizes().slice(0, lead),
+                      op, ": done must be ", q.sizes().slice(0, lead),
+                      " on q's device");
+  }
+  if (state.defined()) {
+    TORCH_CHECK_TYPE(state.scalar_type() == torch::kFloat32, op,
+                     ": the state must be fp32, not ", state.scalar_type());
+    TORCH_CHECK_VALUE(state.device() == q.device() && state.dim() == 4 &&
+                          state.size(0) == s.B && state.size(1) == s.H &&
+                          state.size(2) == s.dk && state.size(3) == s.dv,
+                      op, ": the state must be (B, H, dk, dv) on q's device, "
+                      "not ", state.sizes());
+  }
   return s;
 }
 
-const float* check_state(const OptTensor& t, const Tensor& q,
-                         const AttnShape& s, const char* name) {
-  if (!t.has_value()) return nullptr;
-  TORCH_CHECK(t->device() == q.device() &&
-                  t->scalar_type() == torch::kFloat32 &&
-                  t->is_contiguous() && t->dim() == 4 &&
-                  t->size(0) == s.B && t->size(1) == s.H &&
-                  t->size(2) == s.dk && t->size(3) == s.dv,
-              "linear_attention: ", name, " must be (B, H, dk, dv) fp32, "
-              "contiguous, on q's device");
-  return t->data_ptr<float>();
+double scale_of(const char* op, c10::optional<double> scale,
+                const AttnShape& s) {
+  if (!scale.has_value()) return 1.0 / std::sqrt((double)s.dk);
+  TORCH_CHECK_VALUE(std::isfinite(*scale), op, ": scale must be finite");
+  return *scale;
 }
 
 AttnOperand operand(const Tensor& t, int lead) {
@@ -255,14 +344,14 @@ int attn_segments(const AttnShape& s, long* seg_len) {
 }
 
 AttnArgs attn_args(const AttnShape& s, const Tensor& g,
-                   const OptTensor& done) {
+                   const Tensor& done) {
   AttnArgs a{};
   a.log_decay = g.data_ptr<float>();
   a.g_stride = g.size(0) > 1 ? g.stride(0) : 0;
-  if (done.has_value()) {
-    a.done = (const unsigned char*)done->data_ptr();
-    a.done_st = done->size(0) > 1 ? done->stride(0) : 0;
-    a.done_sb = done->size(1) > 1 ? done->stride(1) : 0;
+  if (done.defined()) {
+    a.done = (const unsigned char*)done.data_ptr();
+    a.done_st = done.size(0) > 1 ? done.stride(0) : 0;
+    a.done_sb = done.size(1) > 1 ? done.stride(1) : 0;
   }
   a.T = s.T;
   a.B = (int)s.B;
@@ -293,22 +382,29 @@ Tensor attn_entry_states(AttnArgs a, const AttnRole& role,
   return st;
 }
 
+AttnShape shape_of(const Tensor& q, const Tensor& v) {
+  return AttnShape{q.size(0), q.size(1), q.size(2), q.size(3), v.size(3)};
+}
+
 // (out, final state, entry states of segments or none)
-std::vector<OptTensor> linear_attention_fwd(Tensor q, Tensor k, Tensor v,
-                                            Tensor g, OptTensor done,
-                                            OptTensor state, double scale) {
-  const AttnShape s = check_attn(q, k, v, g, done, 2);
-  const float* s0 = check_state(state, q, s, "state");
+std::array<Tensor, 3> attn_fwd(const Tensor& q0, const Tensor& k0,
+                               const Tensor& v0, const Tensor& g,
+                               const Tensor& done, const Tensor& state0,
+                               double scale) {
+  const AttnShape s = shape_of(q0, v0);
+  const c10::DeviceGuard guard(q0.device());
+  const Tensor q = unit(q0), k = unit(k0), v = unit(v0),
+               state = dense(state0);
   const int type = type_code(q, "q");
-  const c10::DeviceGuard guard(q.device());
-  auto out = torch::empty({s.T, s.B, s.H, s.dv}, q.options());
-  auto fin = torch::empty({s.B, s.H, s.dk, s.dv},
-                          q.options().dtype(torch::kFloat32));
-  if (s.B * s.H == 0) return {out, fin, c10::nullopt};
+  Tensor out = torch::empty({s.T, s.B, s.H, s.dv}, q.options());
+  Tensor fin = torch::empty({s.B, s.H, s.dk, s.dv},
+                            q.options().dtype(torch::kFloat32));
+  Tensor entry;
+  if (s.B * s.H == 0) return {out, fin, entry};
   if (s.T == 0) {
-    if (s0) fin.copy_(*state);
+    if (state.defined()) fin.copy_(state);
     else fin.zero_();
-    return {out, fin, c10::nullopt};
+    return {out, fin, entry};
   }
   AttnArgs a = attn_args(s, g, done);
   AttnRole r{};
@@ -322,14 +418,13 @@ std::vector<OptTensor> linear_attention_fwd(Tensor q, Tensor k, Tensor v,
   r.u_scale = 1.f;
   r.sx = s.dv;
   r.sy = 1;
-  r.s_in = s0;
+  r.s_in = (const float*)ptr(state);
   r.s_out = fin.data_ptr<float>();
   const bool vec = can_vec(q, r.a) && can_vec(k, r.b) && can_vec(v, r.c);
   hipStream_t stream = stream_here();
-  OptTensor entry;
   if (a.nseg > 1) {
-    entry = attn_entry_states(a, r, s0, type, vec, q, stream);
-    r.s_in = entry->data_ptr<float>();
+    entry = attn_entry_states(a, r, r.s_in, type, vec, q, stream);
+    r.s_in = entry.data_ptr<float>();
   }
   a.nroles = 1;
   a.role[0] = r;
@@ -338,121 +433,178 @@ std::vector<OptTensor> linear_attention_fwd(Tensor q, Tensor k, Tensor v,
   return {out, fin, entry};
 }
 
-// (dq, dk, dv, gradient of the state or none)
-std::vector<OptTensor> linear_attention_bwd(
-    Tensor q, Tensor k, Tensor v, Tensor g, OptTensor done, OptTensor state,
-    OptTensor entry, Tensor d_out, OptTensor d_final, double scale,
-    bool need_dstate) {
-  const AttnShape s = check_attn(q, k, v, g, done, 2);
-  const float* s0 = check_state(state, q, s, "state");
-  const float* df = check_state(d_final, q, s, "the final state's gradient");
-  check_unit(d_out, "the output's gradient");
-  TORCH_CHECK(d_out.sizes() == v.sizes() && d_out.device() == q.device() &&
-                  d_out.scalar_type() == q.scalar_type(),
-              "linear_attention: the output's gradient must match the output");
-  const int type = type_code(q, "q");
-  const c10::DeviceGuard guard(q.device());
-  auto dq = torch::empty(q.sizes(), q.options());
-  auto dk = torch::empty(q.sizes(), q.options());
-  auto dv = torch::empty(v.sizes(), q.options());
-  for (auto* t : {&dq, &dk, &dv}) TORCH_CHECK(t->is_contiguous());
-  OptTensor ds;
-  if (need_dstate)
-    ds = torch::empty({s.B, s.H, s.dk, s.dv},
-                      q.options().dtype(torch::kFloat32));
-  if (s.B * s.H == 0) return {dq, dk, dv, ds};
-  if (s.T == 0) {
-    if (need_dstate) {
-      if (df) ds->copy_(*d_final);
-      else ds->zero_();
-    }
-    return {dq, dk, dv, ds};
+class LinearAttention : public torch::autograd::Function<LinearAttention> {
+ public:
+  static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k,
+                               Tensor v, Tensor g, OptTensor done_,
+                               OptTensor state_, double scale) {
+    const Tensor done = or_undefined(done_), state = or_undefined(state_);
+    ctx->set_materialize_grads(false);
+    auto [out, fin, entry] = attn_fwd(q, k, v, g, done, state, scale);
+    ctx->save_for_backward({q, k, v, g, done, state, entry});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["ds"] = state.defined() && state.requires_grad();
+    return {out, fin};
   }
-  AttnArgs a = attn_args(s, g, done);
-  const long heads = s.B * s.H, size = s.dk * s.dv;
-  if (a.nseg > 1)
-    TORCH_CHECK(entry.has_value() && entry->device() == q.device() &&
-                    entry->scalar_type() == torch::kFloat32 &&
-                    entry->is_contiguous() &&
-                    entry->numel() == a.nseg * heads * size,
-                "linear_attention: saved entry states do not match");
-  const AttnOperand oq = operand(q, 2), ok = operand(k, 2),
-                    ov = operand(v, 2), od = operand(d_out, 2);
-  const bool vec = can_vec(q, oq) && can_vec(k, ok) && can_vec(v, ov) &&
-                   can_vec(d_out, od);
-  hipStream_t stream = stream_here();
 
-  AttnRole rv{};   // dv: a = k, b = q, c = d_out, from the last step
-  rv.a = ok;
-  rv.b = oq;
-  rv.c = od;
-  rv.out = dv.data_ptr();
-  rv.dk = (int)s.dk;
-  rv.dv = (int)s.dv;
-  rv.rev = 1;
-  rv.p_scale = rv.u_scale = (float)scale;
-  rv.in_scale = 1.f;
-  rv.s_in = df;
-  rv.sx = s.dv;
-  rv.sy = 1;
-  rv.s_out = need_dstate ? ds->data_ptr<float>() : nullptr;
-  Tensor back;
-  if (a.nseg > 1) {
-    back = attn_entry_states(a, rv, df, type, vec, q, stream);
-    rv.s_in = back.data_ptr<float>();
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const bool need_ds = ctx->saved_data["ds"].toBool();
+    if (!grads[0].defined() && !grads[1].defined())
+      return variable_list(7);
+    const AttnShape s = shape_of(saved[0], saved[2]);
+    const c10::DeviceGuard guard(saved[0].device());
+    const Tensor q = unit(saved[0]), k = unit(saved[1]), v = unit(saved[2]);
+    const Tensor &g = saved[3], &done = saved[4], &entry = saved[6];
+    const Tensor state = dense(saved[5]);
+    const Tensor d_out = grads[0].defined()
+                             ? unit(grads[0])
+                             : torch::zeros(v.sizes(), v.options());
+    const Tensor d_final = dense(grads[1]);
+    const int type = type_code(q, "q");
+    Tensor dq = torch::empty(q.sizes(), q.options());
+    Tensor dk = torch::empty(q.sizes(), q.options());
+    Tensor dv = torch::empty(v.sizes(), q.options());
+    Tensor ds;
+    if (need_ds)
+      ds = torch::empty({s.B, s.H, s.dk, s.dv},
+                        q.options().dtype(torch::kFloat32));
+    if (s.B * s.H > 0 && s.T > 0) {
+      AttnArgs a = attn_args(s, g, done);
+      const AttnOperand oq = operand(q, 2), ok = operand(k, 2),
+                        ov = operand(v, 2), od = operand(d_out, 2);
+      const bool vec = can_vec(q, oq) && can_vec(k, ok) && can_vec(v, ov) &&
+                       can_vec(d_out, od);
+      hipStream_t stream = stream_here();
+      AttnRole rv{};   // dv: a = k, b = q, c = d_out, from the last step
+      rv.a = ok;
+      rv.b = oq;
+      rv.c = od;
+      rv.out = dv.data_ptr();
+      rv.dk = (int)s.dk;
+      rv.dv = (int)s.dv;
+      rv.rev = 1;
+      rv.p_scale = rv.u_scale = (float)scale;
+      rv.in_scale = 1.f;
+      rv.s_in = (const float*)ptr(d_final);
+      rv.sx = s.dv;
+      rv.sy = 1;
+      rv.s_out = need_ds ? ds.data_ptr<float>() : nullptr;
+      Tensor back;
+      if (a.nseg > 1) {
+        back = attn_entry_states(a, rv, rv.s_in, type, vec, q, stream);
+        rv.s_in = back.data_ptr<float>();
+      }
+      AttnRole rk = rv;   // dk: a = v, b = d_out, c = q, the state turned
+      rk.a = ov;
+      rk.b = od;
+      rk.c = oq;
+      rk.out = dk.data_ptr();
+      rk.dk = (int)s.dv;
+      rk.dv = (int)s.dk;
+      rk.sx = 1;
+      rk.sy = s.dv;
+      rk.s_out = nullptr;
+      AttnRole rq{};      // dq: a = d_out, b = v, c = k, from the first step
+      rq.a = od;
+      rq.b = ov;
+      rq.c = ok;
+      rq.out = dq.data_ptr();
+      rq.dk = (int)s.dv;
+      rq.dv = (int)s.dk;
+      rq.p_scale = rq.in_scale = (float)scale;
+      rq.u_scale = 1.f;
+      rq.s_in = (const float*)ptr(a.nseg > 1 ? entry : state);
+      rq.sx = 1;
+      rq.sy = s.dv;
+      a.nroles = 3;
+      a.role[0] = rv;
+      a.role[1] = rk;
+      a.role[2] = rq;
+      launch_attn_chunks(type, &a, vec, 0, stream);
+      check_launch("linear_attention backward");
+    } else if (need_ds && s.B * s.H > 0) {
+      if (d_final.defined()) ds.copy_(d_final);
+      else ds.zero_();
+    }
+    return once({dq, dk, dv, Tensor(), Tensor(), ds, Tensor()},
+                "linear_attention");
   }
-  AttnRole rk = rv;   // dk: a = v, b = d_out, c = q; the same state turned
-  rk.a = ov;
-  rk.b = od;
-  rk.c = oq;
-  rk.out = dk.data_ptr();
-  rk.dk = (int)s.dv;
-  rk.dv = (int)s.dk;
-  rk.sx = 1;
-  rk.sy = s.dv;
-  rk.s_out = nullptr;
-  AttnRole rq{};      // dq: a = d_out, b = v, c = k, from the first step
-  rq.a = od;
-  rq.b = ov;
-  rq.c = ok;
-  rq.out = dq.data_ptr();
-  rq.dk = (int)s.dv;
-  rq.dv = (int)s.dk;
-  rq.p_scale = rq.in_scale = (float)scale;
-  rq.u_scale = 1.f;
-  rq.s_in = a.nseg > 1 ? entry->data_ptr<float>() : s0;
-  rq.sx = 1;
-  rq.sy = s.dv;
-  a.nroles = 3;
-  a.role[0] = rv;
-  a.role[1] = rk;
-  a.role[2] = rq;
-  launch_attn_chunks(type, &a, vec, 0, stream);
-  check_launch("linear_attention backward");
-  return {dq, dk, dv, ds};
+};
+
+std::tuple<Tensor, Tensor> linear_attention(Tensor q, Tensor k, Tensor v,
+                                            Tensor g, OptTensor done_,
+                                            OptTensor state_,
+                                            c10::optional<double> scale_) {
+  const Tensor done = or_undefined(done_), state = or_undefined(state_);
+  const AttnShape s =
+      check_attn("linear_attention", q, k, v, g, done, state, 2);
+  const double scale = scale_of("linear_attention", scale_, s);
+  if (wants_grad({q, k, v, state})) {
+    auto r = LinearAttention::apply(q, k, v, g, done_, state_, scale);
+    return {r[0], r[1]};
+  }
+  auto [out, fin, entry] = attn_fwd(q, k, v, g, done, state, scale);
+  return {out, fin};
+}
+
+bool heads_contiguous(const Tensor& t) {
+  return t.numel() == 0 || t.select(0, 0).is_contiguous();
+}
+
+// first byte and the byte behind the last
+std::pair<uintptr_t, uintptr_t> span_of(const Tensor& t) {
+  long n = 0;
+  for (int i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+  const uintptr_t p = (uintptr_t)t.data_ptr();
+  return {p, p + (n + 1) * t.element_size()};
 }
 
 // q, k (B, H, dk), v (B, H, dv); the states' environments may lie apart
-Tensor linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor g,
-                             Tensor state, Tensor out_state, OptTensor done,
-                             double scale) {
-  const AttnShape s = check_attn(q, k, v, g, done, 1);
-  const int type = type_code(q, "q");
-  for (const Tensor* t : {&state, &out_state}) {
-    TORCH_CHECK(t->device() == q.device() && t->dim() == 4 &&
-                    t->scalar_type() == torch::kFloat32 &&
-                    t->size(0) == s.B && t->size(1) == s.H &&
-                    t->size(2) == s.dk && t->size(3) == s.dv &&
-                    (s.B * s.H == 0 || t->select(0, 0).is_contiguous()),
-                "linear_attention_step: states must be (B, H, dk, dv) fp32 "
-                "on q's device, an environment's heads contiguous");
+std::tuple<Tensor, Tensor> linear_attention_step(
+    Tensor q0, Tensor k0, Tensor v0, Tensor g, Tensor state, OptTensor done_,
+    c10::optional<double> scale_, OptTensor out_state_) {
+  const char* op = "linear_attention_step";
+  const Tensor done = or_undefined(done_);
+  const AttnShape s = check_attn(op, q0, k0, v0, g, done, state, 1);
+  const double scale = scale_of(op, scale_, s);
+  TORCH_CHECK(!wants_grad({q0, k0, v0, state}), op,
+              " has no gradient; use linear_attention with T = 1");
+  const c10::DeviceGuard guard(q0.device());
+  Tensor next;
+  if (out_state_.has_value()) {
+    next = *out_state_;
+    TORCH_CHECK_TYPE(next.scalar_type() == torch::kFloat32, op,
+                     ": out_state must be fp32, not ", next.scalar_type());
+    TORCH_CHECK_VALUE(next.sizes() == state.sizes() &&
+                          next.device() == state.device(),
+                      op, ": out_state must match the state");
+    TORCH_CHECK(!wants_grad({next}), op,
+                " writes out_state in place; it must not require grad");
+    if (next.numel()) {
+      TORCH_CHECK_VALUE(heads_contiguous(next) &&
+                            (s.B == 1 ||
+                             next.stride(0) >= s.H * s.dk * s.dv),
+                        op, ": out_state needs an environment's heads "
+                        "contiguous and environments that do not overlap");
+      if (next.data_ptr() != state.data_ptr() ||
+          next.strides() != state.strides()) {
+        const auto [a0, a1] = span_of(state);
+        const auto [b0, b1] = span_of(next);
+        TORCH_CHECK_VALUE(a1 <= b0 || b1 <= a0, op, ": out_state overlaps "
+                          "the state without being it");
+      }
+    }
+    // autograd has to see the write: the state may be saved somewhere
+    if (!next.is_inference()) next.unsafeGetTensorImpl()->bump_version();
+  } else {
+    next = torch::empty({s.B, s.H, s.dk, s.dv}, state.options());
   }
-  const c10::DeviceGuard guard(q.device());
-  auto out = torch::empty({s.B, s.H, s.dv}, q.options());
-  if (s.B * s.H == 0) return out;
-  TORCH_CHECK(s.B * s.H <= MAX_GRID, "linear_attention_step: batch too large");
-  TORCH_CHECK(s.B == 1 || out_state.stride(0) >= s.H * s.dk * s.dv,
-              "linear_attention_step: environments of the new state overlap");
+  if (!heads_contiguous(state)) state = state.contiguous();
+  const Tensor q = unit(q0), k = unit(k0), v = unit(v0);
+  Tensor out = torch::empty({s.B, s.H, s.dv}, q.options());
+  if (s.B * s.H == 0) return {out, next};
   AttnStepArgs a{};
   a.q = operand(q, 1);
   a.k = operand(k, 1);
@@ -460,14 +612,14 @@ Tensor linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor g,
   a.out = out.data_ptr();
   a.log_decay = g.data_ptr<float>();
   a.g_stride = s.H > 1 ? g.stride(0) : 0;
-  if (done.has_value()) {
-    a.done = (const unsigned char*)done->data_ptr();
-    a.done_sb = s.B > 1 ? done->stride(0) : 0;
+  if (done.defined()) {
+    a.done = (const unsigned char*)done.data_ptr();
+    a.done_sb = s.B > 1 ? done.stride(0) : 0;
   }
   a.s = state.data_ptr<float>();
-  a.d = out_state.data_ptr<float>();
+  a.d = next.data_ptr<float>();
   a.s_sb = s.B > 1 ? state.stride(0) : 0;
-  a.d_sb = s.B > 1 ? out_state.stride(0) : 0;
+  a.d_sb = s.B > 1 ? next.stride(0) : 0;
   a.scale = (float)scale;
   a.B = (int)s.B;
   a.H = (int)s.H;
@@ -476,9 +628,9 @@ Tensor linear_attention_step(Tensor q, Tensor k, Tensor v, Tensor g,
   const bool vec = s.dv % 4 == 0 && ((uintptr_t)a.s & 15) == 0 &&
                    ((uintptr_t)a.d & 15) == 0 && a.s_sb % 4 == 0 &&
                    a.d_sb % 4 == 0;
-  launch_attn_step(type, &a, vec, stream_here());
-  check_launch("linear_attention_step");
-  return out;
+  launch_attn_step(type_code(q, "q"), &a, vec, stream_here());
+  check_launch(op);
+  return {out, next};
 }
 
 // ---------------------------------------------------------------------------
@@ -492,30 +644,45 @@ int scale_exp(long n) {
   return e < 13 ? e : 13;
 }
 
-// tiles of one product of one matrix, and the blocks that share a tile's k
-void plan_product(ns::Args& a, int mode, int tile) {
+// tiles of one product of all matrices, and the blocks that share a tile's k;
+// returns the floats that the parts of split tiles need
+long plan_product(ns::Args& a, int mode, int tile) {
   const int ks = tile == 64 ? 64 : 32;
-  long total = 0;
+  // blocks that run at once: two a CU fit its LDS
+  const long slots = 512;
+  long total = 0, work = 0, longest = 0;
   for (int i = 0; i < a.count; ++i) {
     ns::Mat& m = a.mat[i];
     const int tm = m.mp / tile, tn = m.np / tile;
     m.tiles = mode == 2 ? tm * tn : tm * (tm + 1) / 2;
+    const long steps = (mode == 0 ? m.np : m.mp) / ks;
     total += m.tiles;
+    work += m.tiles * steps;
+    longest = std::max(longest, steps);
   }
-  int blocks = 0;
+  // Steps of k for a block so that all blocks run at once, 512 values at
+  // least: below that, adding the parts costs more than it saves. Nothing is
+  // split where the blocks fill the card anyway or the gain is small.
+  long per = std::max((work + slots - 1) / slots, 512L / ks);
+  if (total >= slots || longest * 2 <= per * 3) per = longest;
+  long part = 0;
+  int blocks = 0, sums = 0;
   for (int i = 0; i < a.count; ++i) {
     ns::Mat& m = a.mat[i];
-    // two blocks a CU fit; a block keeps 256 values of k at least, so that
-    // adding the parts does not outweigh them
     const long steps = (mode == 0 ? m.np : m.mp) / ks;
-    long s = total >= 512 ? 1 : 512 / total;
-    const long most = steps * ks / 256;
-    if (s > most) s = most;
-    m.splits = (int)(s < 1 ? 1 : s);
+    m.splits = (int)((steps + per - 1) / per);
     a.first[i] = blocks;
+    a.first_sum[i] = sums;
+    a.part_off[i] = part;
     blocks += m.tiles * m.splits;
+    if (m.splits > 1) {
+      sums += m.tiles;
+      part += (long)m.tiles * m.splits * tile * tile;
+    }
   }
   a.first[a.count] = blocks;
+  a.first_sum[a.count] = sums;
+  return part;
 }
 
 void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
@@ -579,28 +746,26 @@ void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
       m.b = m.a + square;
       parts = m.b + square;
     }
-    long partial = 1, arrived = 1;
-    for (int mode = 0; mode < 3; ++mode) {
-      plan_product(a, mode, tile);
-      long p = 0, n = 0;
-      for (int i = 0; i < a.count; ++i) {
-        n += a.mat[i].tiles;
-        if (a.mat[i].splits > 1)
-          p += (long)a.mat[i].tiles * a.mat[i].splits * tile * tile;
-      }
-      partial = p > partial ? p : partial;
-      arrived = n > arrived ? n : arrived;
+    int norm_blocks = 0;
+    for (int i = 0; i < a.count; ++i) {
+      ns::Mat& m = a.mat[i];
+      const long want = ((long)m.m * m.n + 8191) / 8192;
+      m.norm_blocks = (int)std::min(want, (long)ns::MAX_NORM_BLOCKS);
+      a.first_norm[i] = norm_blocks;
+      norm_blocks += m.norm_blocks;
     }
+    a.first_norm[a.count] = norm_blocks;
+    long partial = 0;
+    for (int mode = 0; mode < 3; ++mode)
+      partial = std::max(partial, plan_product(a, mode, tile));
     auto work = torch::empty({parts}, like.options().dtype(torch::kFloat16));
     auto split = torch::empty({partial},
                               like.options().dtype(torch::kFloat32));
-    auto count = torch::zeros({arrived}, like.options().dtype(torch::kInt32));
-    auto sums = torch::empty({(long)a.count * ns::NORM_BLOCKS},
+    auto sums = torch::empty({norm_blocks},
                              like.options().dtype(torch::kFloat64));
     auto rho = torch::empty({a.count}, like.options().dtype(torch::kFloat32));
     a.parts = (_Float16*)work.data_ptr();
     a.partial = split.data_ptr<float>();
-    a.arrived = count.data_ptr<int>();
     a.sums = sums.data_ptr<double>();
     a.rho = rho.data_ptr<float>();
     a.eps = eps;
@@ -610,15 +775,6 @@ void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
       a.last = k + 1 == steps;
       for (int mode = 0; mode < 3; ++mode) {
         plan_product(a, mode, tile);
-        long p = 0;
-        int n = 0;
-        for (int i = 0; i < a.count; ++i) {
-          a.part_off[i] = p;
-          a.arrive_off[i] = n;
-          n += a.mat[i].tiles;
-          if (a.mat[i].splits > 1)
-            p += (long)a.mat[i].tiles * a.mat[i].splits * tile * tile;
-        }
         launch_ns_product(mode, tile, &a, stream);
       }
     }
@@ -631,20 +787,14 @@ void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
 void register_core_ops(pybind11::module_& m) {
   m.def("orthogonalize", &orthogonalize, py::arg("src"), py::arg("dst"),
         py::arg("steps"), py::arg("eps"));
-  m.def("linear_attention_fwd", &linear_attention_fwd, py::arg("q"),
-        py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("done"),
-        py::arg("state"), py::arg("scale"));
-  m.def("linear_attention_bwd", &linear_attention_bwd, py::arg("q"),
-        py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("done"),
-        py::arg("state"), py::arg("entry"), py::arg("d_out"),
-        py::arg("d_final"), py::arg("scale"), py::arg("need_dstate"));
+  m.def("linear_attention", &linear_attention, py::arg("q"), py::arg("k"),
+        py::arg("v"), py::arg("log_decay"), py::arg("done") = py::none(),
+        py::arg("state") = py::none(), py::arg("scale") = py::none());
   m.def("linear_attention_step", &linear_attention_step, py::arg("q"),
         py::arg("k"), py::arg("v"), py::arg("log_decay"), py::arg("state"),
-        py::arg("out_state"), py::arg("done"), py::arg("scale"));
-  m.def("layer_norm_fwd", &layer_norm_fwd, py::arg("x"),
+        py::arg("done") = py::none(), py::arg("scale") = py::none(),
+        py::arg("out_state") = py::none());
+  m.def("layer_norm", &layer_norm, py::arg("x"),
         py::arg("weight") = py::none(), py::arg("bias") = py::none(),
-        py::arg("eps") = 1e-5, py::arg("save") = false);
-  m.def("layer_norm_bwd", &layer_norm_bwd, py::arg("dy"), py::arg("x"),
-        py::arg("weight"), py::arg("stats"), py::arg("need_dx"),
-        py::arg("need_dw"), py::arg("need_db"), py::arg("param_fp32"));
+        py::arg("eps") = 1e-5);
 }

@@ -5,7 +5,7 @@ namespace impala {
 namespace ortho {
 
 constexpr int MAX_MATS = 24;   // of one launch; all fit the kernel's arguments
-constexpr int NORM_BLOCKS = 64;
+constexpr int MAX_NORM_BLOCKS = 256;   // of one matrix
 
 // One matrix, worked on as m x n with m <= n (a tall one is turned), both
 // padded with zeros to whole tiles. Offsets are in elements of the workspace
@@ -19,6 +19,7 @@ struct Mat {
   int m, n, mp, np;
   int ex, ea;              // exponents of the scales of X, and of A and b
   int type;
+  int norm_blocks;
   int tiles, splits;       // of the launch at hand
 };
 
@@ -26,12 +27,12 @@ struct Args {
   Mat mat[MAX_MATS];
   int count;
   int first[MAX_MATS + 1];   // blocks before a matrix's own
+  int first_sum[MAX_MATS + 1];   // the same of the launch that adds parts
+  int first_norm[MAX_MATS + 1];
   _Float16* parts;
   float* partial;            // split products
   long part_off[MAX_MATS];   //   of a matrix, in floats
-  int* arrived;              //   blocks of a tile that are done, zero between
-  int arrive_off[MAX_MATS];
-  double* sums;              // (count, NORM_BLOCKS) sums of squares
+  double* sums;              // sums of squares, a matrix's blocks in a row
   float* rho;                // |g| / (|g| + eps)
   double eps;
   int round, last;

@@ -8,8 +8,9 @@
 // above 1.21, so X is bounded all along. A tall matrix is worked on turned.
 //
 // Bound: matrix products for wide layers, latency for the small matrices of
-// the policy nets, so one launch does one product of all matrices of a list
-// (two launches to start, three a round).
+// the policy nets, so one launch does one product of all matrices of a list:
+// two launches to start and three a round, and one more for a product whose
+// few tiles are split along a long k.
 //
 // The products run on the fp16 matrix cores with fp32 accuracy: an operand is
 // kept as two fp16 parts, hi + lo = 22 bits, and a product is hi hi + hi lo +
@@ -51,9 +52,9 @@ __device__ inline void store_any(void* p, long i, int type, float v) {
   else ((half_t*)p)[i] = (half_t)v;
 }
 
-__device__ inline int mat_of(const Args& a, int block) {
+__device__ inline int mat_of(const int* first, int count, int block) {
   int i = 0;
-  while (i + 1 < a.count && block >= a.first[i + 1]) ++i;
+  while (i + 1 < count && block >= first[i + 1]) ++i;
   return i;
 }
 
@@ -67,33 +68,43 @@ __device__ inline int bound_exp(float rho, int k) {
   return e - 1;
 }
 
+// sum over a block of 256, in every thread
 __device__ inline double block_sum(double v) {
   __shared__ double s[4];
   for (int off = 32; off > 0; off >>= 1) v += __shfl_down(v, off, 64);
   if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
   __syncthreads();
-  return s[0] + s[1] + s[2] + s[3];
+  return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // sums of squares in 64 bits: no overflow for any fp32 gradient, and an order
 // of adding that does not change
 __global__ void __launch_bounds__(256) ns_norm(Args args) {
-  const int mi = blockIdx.x / NORM_BLOCKS, blk = blockIdx.x % NORM_BLOCKS;
+  const int mi = mat_of(args.first_norm, args.count, blockIdx.x);
   const Mat& M = args.mat[mi];
+  const int blk = blockIdx.x - args.first_norm[mi];
   const long total = (long)M.m * M.n;
+  const long stride = (long)M.norm_blocks * 256;
   // the axis that is contiguous in memory runs fastest
   const bool by_i = M.src_i < M.src_j;
   const int fast = by_i ? M.m : M.n;
   const long sf = by_i ? M.src_i : M.src_j, ss = by_i ? M.src_j : M.src_i;
   double acc = 0.0;
-  for (long e = (long)blk * 256 + threadIdx.x; e < total;
-       e += (long)NORM_BLOCKS * 256) {
-    const long s = e / fast, f = e - s * fast;
-    const double v = load_any(M.src, s * ss + f * sf, M.type);
-    acc += v * v;
+  if (sf == 1 && ss == fast) {   // dense: no division an element
+    #pragma unroll 4
+    for (long e = (long)blk * 256 + threadIdx.x; e < total; e += stride) {
+      const double v = load_any(M.src, e, M.type);
+      acc = fma(v, v, acc);
+    }
+  } else {
+    for (long e = (long)blk * 256 + threadIdx.x; e < total; e += stride) {
+      const long s = e / fast, f = e - s * fast;
+      const double v = load_any(M.src, s * ss + f * sf, M.type);
+      acc = fma(v, v, acc);
+    }
   }
   acc = block_sum(acc);
-  if (threadIdx.x == 0) args.sums[mi * NORM_BLOCKS + blk] = acc;
+  if (threadIdx.x == 0) args.sums[blockIdx.x] = acc;
 }
 
 __device__ inline void split_store(half_t* p, long plane, long at, float v) {
@@ -105,15 +116,16 @@ __device__ inline void split_store(half_t* p, long plane, long at, float v) {
 // G -> parts of X and X^T, 64 x 64 a block
 __global__ void __launch_bounds__(256) ns_prepare(Args args) {
   __shared__ float tile[64][65];
-  const int mi = mat_of(args, blockIdx.x);
+  const int mi = mat_of(args.first, args.count, blockIdx.x);
   const Mat& M = args.mat[mi];
   const int t = blockIdx.x - args.first[mi];
   const int tn = M.np / 64;
   const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
 
-  double sum = 0.0;
-  for (int k = 0; k < NORM_BLOCKS; ++k) sum += args.sums[mi * NORM_BLOCKS + k];
-  const double norm = sqrt(sum);
+  static_assert(MAX_NORM_BLOCKS <= 256, "one partial sum a thread");
+  const double norm = sqrt(block_sum(
+      (int)threadIdx.x < M.norm_blocks
+          ? args.sums[args.first_norm[mi] + threadIdx.x] : 0.0));
   const float rho = (float)(norm / (norm + args.eps));
   const int e = M.ex - bound_exp(rho, 0);
   const double mul = ldexp(1.0 / (norm + args.eps), e);
@@ -144,12 +156,107 @@ __global__ void __launch_bounds__(256) ns_prepare(Args args) {
 }
 
 // --------------------------------------------------------------------------
+// tiles: all of X, or those on and under the diagonal, row by row
+// --------------------------------------------------------------------------
+template <int MODE, int TILE>
+__device__ inline void place(const Mat& M, int tile, int* ti, int* tj) {
+  if (MODE == 2) {
+    const int tn = M.np / TILE;
+    *ti = tile / tn;
+    *tj = tile % tn;
+  } else {
+    int i = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
+    while ((i + 1) * (i + 2) / 2 <= tile) ++i;
+    while (i * (i + 1) / 2 > tile) --i;
+    *ti = i;
+    *tj = tile - i * (i + 1) / 2;
+  }
+}
+
+// a tile's sums -> the polynomial, new parts in both orientations, or the
+// result
+template <int MODE, int TILE>
+__device__ inline void finish(const Args& args, int mi, int ti, int tj,
+                              f32x4 (&acc)[TILE / 32][TILE / 32]) {
+  constexpr int W = TILE / 2, NF = W / 16;
+  const Mat& M = args.mat[mi];
+  const int l = threadIdx.x & 63, m = l & 15, g = l >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = (wave >> 1) * W, wj = (wave & 1) * W;
+  const int cur = args.round & 1;
+  const float rho = args.rho[mi];
+  const int e_now = bound_exp(rho, args.round);
+  const int sx = M.ex - e_now;               // X   = stored * 2^-sx
+  const int sa = M.ea - 2 * e_now;           // A   = stored * 2^-sa
+  const int sb = M.ea;                       // B   = stored * 2^-sb
+  const int sx2 = M.ex - bound_exp(rho, args.round + 1);
+  half_t* C = args.parts + (MODE == 0 ? M.a : MODE == 1 ? M.b : M.x);
+  half_t* CT = MODE == 2 ? args.parts + M.xt[cur ^ 1] : C;
+  const int ldc = MODE == 2 ? M.np : M.mp;
+  const long plane = MODE == 2 ? (long)M.mp * M.np : (long)M.mp * M.mp;
+  const half_t* Ap = args.parts + M.a;
+  // products of stored values -> stored values. Two factors, so that the
+  // exponents of tiny gradients stay in range
+  const float f1 = MODE == 0 ? ldexpf(1.f, sa - 2 * sx)
+                 : MODE == 1 ? ldexpf(NS_C, -2 * M.ea)
+                             : args.last ? ldexpf(1.f, -sb)
+                                         : ldexpf(1.f, sx2 - sb - sx);
+  const float f2 = MODE == 1 ? ldexpf(1.f, 4 * e_now + sb)
+                 : MODE == 2 && args.last ? ldexpf(1.f, -sx) : 1.f;
+  const float fb = ldexpf(NS_B, -M.ea + 2 * e_now + sb);
+  const float fa = ldexpf(NS_A, sb);
+
+  #pragma unroll
+  for (int i = 0; i < NF; ++i) {
+    #pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const int row = ti * TILE + wi + 16 * i + 4 * g;   // + r
+      const int col = tj * TILE + wj + 16 * j + m;
+      float v[4];
+      #pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) v[r4] = acc[i][j][r4] * f1 * f2;
+      if constexpr (MODE == 1) {
+        #pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+          const long at = (long)(row + r4) * ldc + col;
+          v[r4] = fmaf(fb, (float)Ap[at] + (float)Ap[at + plane], v[r4]);
+          if (row + r4 == col) v[r4] += fa;
+        }
+      }
+      if (MODE == 2 && args.last) {
+        #pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4)
+          if (row + r4 < M.m && col < M.n)
+            store_any(M.dst, (row + r4) * M.dst_i + col * M.dst_j, M.type,
+                      v[r4]);
+        continue;
+      }
+      halfx4 h, w;
+      #pragma unroll
+      for (int r4 = 0; r4 < 4; ++r4) {
+        h[r4] = (half_t)v[r4];
+        w[r4] = (half_t)(v[r4] - (float)h[r4]);
+        const long at = (long)(row + r4) * ldc + col;
+        C[at] = h[r4];
+        C[at + plane] = w[r4];
+      }
+      if (MODE == 2 || ti != tj) {
+        const long at = (long)col * M.mp + row;
+        *reinterpret_cast<halfx4*>(CT + at) = h;
+        *reinterpret_cast<halfx4*>(CT + at + plane) = w;
+      }
+    }
+  }
+}
+
+// --------------------------------------------------------------------------
 // One product, C = P Q^T over k, P and Q in two parts with k contiguous.
 // MODE 0: A = X X^T. MODE 1: B = a I + b A + c A A. MODE 2: X = B X.
 // TILE x TILE of C a block, four waves of half that each way; k in steps of
 // KS through two LDS buffers, the next step's rows on their way in registers.
-// Few tiles of long k are split; the last block of a tile to arrive adds the
-// parts, in order.
+// Few tiles of long k are split over blocks; a second launch adds their parts
+// (letting the last block of a tile add them costs a write-back of the L2 a
+// block: 175 us against 60 for six matrices of 1024).
 // --------------------------------------------------------------------------
 template <int MODE, int TILE>
 __global__ void __launch_bounds__(256) ns_product(Args args) {
@@ -160,21 +267,12 @@ __global__ void __launch_bounds__(256) ns_product(Args args) {
   constexpr int PER_ROW = KS / 8;
   __shared__ __align__(16) half_t lds[2][4][TILE * LD];
 
-  const int mi = mat_of(args, blockIdx.x);
+  const int mi = mat_of(args.first, args.count, blockIdx.x);
   const Mat& M = args.mat[mi];
   const int id = blockIdx.x - args.first[mi];
   const int tile = id / M.splits, split = id % M.splits;
   int ti, tj;
-  if (MODE == 2) {
-    const int tn = M.np / TILE;
-    ti = tile / tn;
-    tj = tile % tn;
-  } else {   // under the diagonal, row by row
-    ti = (int)((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-    while ((ti + 1) * (ti + 2) / 2 <= tile) ++ti;
-    while (ti * (ti + 1) / 2 > tile) --ti;
-    tj = tile - ti * (ti + 1) / 2;
-  }
+  place<MODE, TILE>(M, tile, &ti, &tj);
   const int cur = args.round & 1;
   const int K = MODE == 0 ? M.np : M.mp;
   const long plane_p = MODE == 0 ? (long)M.mp * M.np : (long)M.mp * M.mp;
@@ -261,11 +359,9 @@ __global__ void __launch_bounds__(256) ns_product(Args args) {
     if (k + 1 < k_hi) put(buf ^ 1);
   }
 
-  if (M.splits > 1) {
-    // leave the part; whoever comes last adds all of the tile
-    float* base = args.partial + args.part_off[mi] +
-                  (long)tile * M.splits * TILE * TILE;
-    float* mine = base + (long)split * TILE * TILE;
+  if (M.splits > 1) {   // ns_sum adds the parts
+    float* mine = args.partial + args.part_off[mi] +
+                  ((long)tile * M.splits + split) * TILE * TILE;
     #pragma unroll
     for (int i = 0; i < NF; ++i) {
       #pragma unroll
@@ -273,110 +369,51 @@ __global__ void __launch_bounds__(256) ns_product(Args args) {
         *reinterpret_cast<f32x4*>(mine + ((i * NF + j) * 256 + tid) * 4) =
             acc[i][j];
     }
-    __threadfence();
-    __syncthreads();
-    int* count = args.arrived + args.arrive_off[mi] + tile;
-    // the flag lies in the operands' LDS, which is free by now: two blocks of
-    // 128 x 128 fill a CU's 160 KB to the byte
-    int* last_block = reinterpret_cast<int*>(&lds[0][0][0]);
-    if (tid == 0)
-      *last_block = __hip_atomic_fetch_add(count, 1, __ATOMIC_ACQ_REL,
-                                           __HIP_MEMORY_SCOPE_AGENT) ==
-                    M.splits - 1;
-    __syncthreads();
-    if (!*last_block) return;
-    __threadfence();
-    #pragma unroll
-    for (int i = 0; i < NF; ++i) {
-      #pragma unroll
-      for (int j = 0; j < NF; ++j) {
-        f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < M.splits; ++s)
-          sum += *reinterpret_cast<const f32x4*>(
-              base + (long)s * TILE * TILE + ((i * NF + j) * 256 + tid) * 4);
-        acc[i][j] = sum;
-      }
-    }
-    if (tid == 0)   // ready for the next launch
-      __hip_atomic_store(count, 0, __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_AGENT);
+    return;
   }
+  finish<MODE, TILE>(args, mi, ti, tj, acc);
+}
 
-  // ---- scales, the polynomial, both orientations
-  const float rho = args.rho[mi];
-  const int e_now = bound_exp(rho, args.round);
-  const int sx = M.ex - e_now;               // X   = stored * 2^-sx
-  const int sa = M.ea - 2 * e_now;           // A   = stored * 2^-sa
-  const int sb = M.ea;                       // B   = stored * 2^-sb
-  const int sx2 = M.ex - bound_exp(rho, args.round + 1);
-  half_t* C = args.parts + (MODE == 0 ? M.a : MODE == 1 ? M.b : M.x);
-  half_t* CT = MODE == 2 ? args.parts + M.xt[cur ^ 1] : C;
-  const int ldc = MODE == 2 ? M.np : M.mp;
-  const long plane = MODE == 2 ? (long)M.mp * M.np : (long)M.mp * M.mp;
-  const half_t* Ap = args.parts + M.a;
-  // products of stored values -> stored values. Two factors, so that the
-  // exponents of tiny gradients stay in range
-  const float f1 = MODE == 0 ? ldexpf(1.f, sa - 2 * sx)
-                 : MODE == 1 ? ldexpf(NS_C, -2 * M.ea)
-                             : args.last ? ldexpf(1.f, -sb)
-                                         : ldexpf(1.f, sx2 - sb - sx);
-  const float f2 = MODE == 1 ? ldexpf(1.f, 4 * e_now + sb)
-                 : MODE == 2 && args.last ? ldexpf(1.f, -sx) : 1.f;
-  const float fb = ldexpf(NS_B, -M.ea + 2 * e_now + sb);
-  const float fa = ldexpf(NS_A, sb);
-
+// the parts of split products, added in order
+template <int MODE, int TILE>
+__global__ void __launch_bounds__(256) ns_sum(Args args) {
+  constexpr int NF = TILE / 32;
+  const int mi = mat_of(args.first_sum, args.count, blockIdx.x);
+  const Mat& M = args.mat[mi];
+  const int tile = blockIdx.x - args.first_sum[mi];
+  int ti, tj;
+  place<MODE, TILE>(M, tile, &ti, &tj);
+  const float* base = args.partial + args.part_off[mi] +
+                      (long)tile * M.splits * TILE * TILE;
+  f32x4 acc[NF][NF];
   #pragma unroll
   for (int i = 0; i < NF; ++i) {
     #pragma unroll
     for (int j = 0; j < NF; ++j) {
-      const int row = ti * TILE + wi + 16 * i + 4 * g;   // + r
-      const int col = tj * TILE + wj + 16 * j + m;
-      float v[4];
-      #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) v[r4] = acc[i][j][r4] * f1 * f2;
-      if constexpr (MODE == 1) {
-        #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const long at = (long)(row + r4) * ldc + col;
-          v[r4] = fmaf(fb, (float)Ap[at] + (float)Ap[at + plane], v[r4]);
-          if (row + r4 == col) v[r4] += fa;
-        }
-      }
-      if (MODE == 2 && args.last) {
-        #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4)
-          if (row + r4 < M.m && col < M.n)
-            store_any(M.dst, (row + r4) * M.dst_i + col * M.dst_j, M.type,
-                      v[r4]);
-        continue;
-      }
-      halfx4 h, w;
-      #pragma unroll
-      for (int r4 = 0; r4 < 4; ++r4) {
-        h[r4] = (half_t)v[r4];
-        w[r4] = (half_t)(v[r4] - (float)h[r4]);
-        const long at = (long)(row + r4) * ldc + col;
-        C[at] = h[r4];
-        C[at + plane] = w[r4];
-      }
-      if (MODE == 2 || ti != tj) {
-        const long at = (long)col * M.mp + row;
-        *reinterpret_cast<halfx4*>(CT + at) = h;
-        *reinterpret_cast<halfx4*>(CT + at + plane) = w;
-      }
+      const float* p = base + ((i * NF + j) * 256 + threadIdx.x) * 4;
+      f32x4 sum = *reinterpret_cast<const f32x4*>(p);
+      for (int s = 1; s < M.splits; ++s)
+        sum += *reinterpret_cast<const f32x4*>(p + (long)s * TILE * TILE);
+      acc[i][j] = sum;
     }
   }
+  finish<MODE, TILE>(args, mi, ti, tj, acc);
+}
+
+template <int MODE, int TILE>
+void run_product(const Args& a, hipStream_t s) {
+  hipLaunchKernelGGL((ns_product<MODE, TILE>), dim3(a.first[a.count]),
+                     dim3(256), 0, s, a);
+  if (a.first_sum[a.count] > 0)
+    hipLaunchKernelGGL((ns_sum<MODE, TILE>), dim3(a.first_sum[a.count]),
+                       dim3(256), 0, s, a);
 }
 
 template <int TILE>
-void run_product(int mode, const Args& a, int blocks, hipStream_t s) {
-  const dim3 grid(blocks), block(256);
-  if (mode == 0)
-    hipLaunchKernelGGL((ns_product<0, TILE>), grid, block, 0, s, a);
-  else if (mode == 1)
-    hipLaunchKernelGGL((ns_product<1, TILE>), grid, block, 0, s, a);
-  else
-    hipLaunchKernelGGL((ns_product<2, TILE>), grid, block, 0, s, a);
+void run_mode(int mode, const Args& a, hipStream_t s) {
+  if (mode == 0) run_product<0, TILE>(a, s);
+  else if (mode == 1) run_product<1, TILE>(a, s);
+  else run_product<2, TILE>(a, s);
 }
 
 }  // namespace ortho
@@ -387,7 +424,7 @@ using namespace impala::ortho;
 extern "C" {
 
 void launch_ns_start(Args* a, hipStream_t s) {
-  hipLaunchKernelGGL(ns_norm, dim3(a->count * NORM_BLOCKS), dim3(256), 0, s,
+  hipLaunchKernelGGL(ns_norm, dim3(a->first_norm[a->count]), dim3(256), 0, s,
                      *a);
   int n = 0;
   for (int i = 0; i < a->count; ++i) {
@@ -398,11 +435,10 @@ void launch_ns_start(Args* a, hipStream_t s) {
   hipLaunchKernelGGL(ns_prepare, dim3(n), dim3(256), 0, s, *a);
 }
 
-// the caller has set tiles, splits and first
+// the caller has planned the product: tiles, splits and their blocks
 void launch_ns_product(int mode, int tile, const Args* a, hipStream_t s) {
-  const int blocks = a->first[a->count];
-  if (tile == 64) run_product<64>(mode, *a, blocks, s);
-  else run_product<128>(mode, *a, blocks, s);
+  if (tile == 64) run_mode<64>(mode, *a, s);
+  else run_mode<128>(mode, *a, s);
 }
 
 }  // extern "C"

@@ -61,6 +61,14 @@ def hip_available() -> bool:
     return ext_hip(required=True) is not None
 
 
+def ext_for(t: torch.Tensor):
+    """The kernels' extension where ``t`` lies on a GPU and eager ops are not
+    forced, else None. The cheap form of hip_available() for small calls."""
+    if not t.is_cuda or _eager_forced():
+        return None
+    return _EXT_HIP or ext_hip()
+
+
 def pin_host_memory(t: torch.Tensor):
     """hipHostRegister a CPU tensor's storage (page-lock for async DMA).
 

@@ -13,7 +13,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from torched_impala_amd import ops
 
@@ -21,6 +20,8 @@ _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
 def _check(x, weight, bias, eps):
+    """What the kernels' host side (csrc/core_ops.cpp) checks, for the eager
+    path."""
     if x.dtype not in _TYPES:
         raise TypeError(f"layer_norm: x must be fp32, bf16 or fp16, "
                         f"not {x.dtype}")
@@ -46,39 +47,6 @@ def _check(x, weight, bias, eps):
                          f"not {eps}")
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """(rows, cols) with unit column stride: a view where strides allow."""
-    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    if x.shape[1] > 1 and x.stride(1) != 1:
-        x = x.contiguous()
-    return x
-
-
-class _LayerNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        w = weight.contiguous() if weight is not None else None
-        b = bias.contiguous() if bias is not None else None
-        y, stats = ops.ext_hip().layer_norm_fwd(_rows(x), w, b, eps, True)
-        # x itself is saved, not its 2-D view, so that an in-place change
-        # of it before backward is caught
-        ctx.save_for_backward(x, w, stats)
-        p = bias if weight is None else weight
-        ctx.param_fp32 = p is None or p.dtype is torch.float32
-        return y.view(x.shape)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, w, stats = ctx.saved_tensors
-        nx, nw, nb = ctx.needs_input_grad[:3]
-        xr = _rows(x)
-        dx, dw, db = ops.ext_hip().layer_norm_bwd(
-            dy.reshape(xr.shape).contiguous(), xr, w, stats, nx, nw, nb,
-            ctx.param_fp32)
-        return (dx.view(x.shape) if nx else None), dw, db, None
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5,
@@ -92,20 +60,13 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     in x, weight and bias. ``force_eager`` takes torch's ops instead of the
     kernels. Raises TypeError or ValueError for anything else.
     """
+    ext = None if force_eager else ops.ext_for(x)
+    if ext is not None:   # checks, saves and differentiates by itself
+        return ext.layer_norm(x, weight, bias, eps)
+    # eager fallback (CPU tests / escape hatch) — same math
     _check(x, weight, bias, eps)
-    if force_eager or not (x.is_cuda and ops.hip_available()):
-        # eager fallback (CPU tests / escape hatch) — same math
-        f32 = torch.float32
-        return torch.nn.functional.layer_norm(
-            x.to(f32), x.shape[-1:],
-            None if weight is None else weight.to(f32),
-            None if bias is None else bias.to(f32), eps).to(x.dtype)
-    if torch.is_grad_enabled() and (
-            x.requires_grad
-            or (weight is not None and weight.requires_grad)
-            or (bias is not None and bias.requires_grad)):
-        return _LayerNorm.apply(x, weight, bias, float(eps))
-    y, _ = ops.ext_hip().layer_norm_fwd(
-        _rows(x), None if weight is None else weight.contiguous(),
-        None if bias is None else bias.contiguous(), float(eps), False)
-    return y.view(x.shape)
+    f32 = torch.float32
+    return torch.nn.functional.layer_norm(
+        x.to(f32), x.shape[-1:],
+        None if weight is None else weight.to(f32),
+        None if bias is None else bias.to(f32), eps).to(x.dtype)

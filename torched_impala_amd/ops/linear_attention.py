@@ -18,7 +18,6 @@ import math
 from typing import Optional, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from torched_impala_amd import ops
 
@@ -27,7 +26,8 @@ MAX_HEAD = 128
 
 
 def _check(name, q, k, v, log_decay, done, state, scale, lead):
-    """Shapes, types and devices of a call; returns the scale."""
+    """Shapes, types and devices of a call, as the kernels' host side
+    (csrc/core_ops.cpp) checks them, for the eager path; returns the scale."""
     if q.dtype not in _TYPES:
         raise TypeError(f"{name}: q must be fp32, bf16 or fp16, "
                         f"not {q.dtype}")
@@ -84,41 +84,6 @@ def _check(name, q, k, v, log_decay, done, state, scale, lead):
     return float(scale)
 
 
-def _unit(t: torch.Tensor) -> torch.Tensor:
-    """A head's features side by side; every other stride is free."""
-    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-class _LinearAttention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, done, state, scale):
-        ctx.set_materialize_grads(False)
-        out, final, entry = ops.ext_hip().linear_attention_fwd(
-            _unit(q), _unit(k), _unit(v), log_decay, done,
-            None if state is None else state.contiguous(), scale)
-        ctx.save_for_backward(q, k, v, log_decay, done, state, entry)
-        ctx.scale = scale
-        return out, final
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_out, d_final):
-        q, k, v, log_decay, done, state, entry = ctx.saved_tensors
-        if d_out is None and d_final is None:
-            return (None,) * 7
-        if d_out is None:
-            d_out = torch.zeros((), dtype=q.dtype, device=q.device
-                                ).expand(v.shape).contiguous()
-        need_state = state is not None and ctx.needs_input_grad[5]
-        dq, dk, dv, ds = ops.ext_hip().linear_attention_bwd(
-            _unit(q), _unit(k), _unit(v), log_decay, done,
-            None if state is None else state.contiguous(), entry,
-            _unit(d_out),
-            None if d_final is None else d_final.contiguous(),
-            ctx.scale, need_state)
-        return dq, dk, dv, None, None, ds, None
-
-
 def _eager(q, k, v, log_decay, done, state, scale):
     """The recurrence in fp32 torch ops (CPU tests / escape hatch)."""
     T, B, H, dk = q.shape
@@ -165,24 +130,18 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     step or another episode. Raises TypeError or ValueError for anything
     else.
     """
+    ext = None if force_eager else ops.ext_for(q)
+    if ext is not None:   # checks, saves and differentiates by itself
+        return ext.linear_attention(q, k, v, log_decay, done, state, scale)
     scale = _check("linear_attention", q, k, v, log_decay, done, state,
                    scale, 2)
-    if force_eager or not (q.is_cuda and ops.hip_available()):
-        return _eager(q, k, v, log_decay, done, state, scale)
-    if torch.is_grad_enabled() and (
-            q.requires_grad or k.requires_grad or v.requires_grad
-            or (state is not None and state.requires_grad)):
-        return _LinearAttention.apply(q, k, v, log_decay, done, state, scale)
-    out, final, _ = ops.ext_hip().linear_attention_fwd(
-        _unit(q), _unit(k), _unit(v), log_decay, done,
-        None if state is None else state.contiguous(), scale)
-    return out, final
+    return _eager(q, k, v, log_decay, done, state, scale)
 
 
 def _span(t: torch.Tensor):
-    """First and last byte of a tensor's memory (non-empty tensors)."""
+    """First byte of a tensor's memory and the byte behind the last."""
     n = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
 
 
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -200,6 +159,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     contiguous. Not differentiable: raises RuntimeError where a gradient is
     asked for (``linear_attention`` with T = 1 has one).
     """
+    ext = ops.ext_for(q)
+    if ext is not None:
+        return ext.linear_attention_step(q, k, v, log_decay, state, done,
+                                         scale, out_state)
     scale = _check("linear_attention_step", q, k, v, log_decay, done, state,
                    scale, 1)
     if torch.is_grad_enabled() and any(
@@ -230,27 +193,14 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             if not same:
                 a0, a1 = _span(state)
                 b0, b1 = _span(out_state)
-                if a0 <= b1 and b0 <= a1:
+                if a0 < b1 and b0 < a1:
                     raise ValueError("linear_attention_step: out_state "
                                      "overlaps the state without being it")
-    if not (q.is_cuda and ops.hip_available()):
-        with torch.no_grad():
-            out, new = _eager(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0),
-                              log_decay,
-                              None if done is None else done.unsqueeze(0),
-                              state, scale)
-            if out_state is not None:
-                new = out_state.copy_(new)
-        return out[0], new
-    if state.numel() and not state[0].is_contiguous():
-        state = state.contiguous()
-    if out_state is None:
-        out_state = torch.empty(state.shape, dtype=torch.float32,
-                                device=state.device)
-    elif not out_state.is_inference():
-        # autograd has to see the write: the state may be saved somewhere
-        torch.autograd.graph.increment_version(out_state)
-    out = ops.ext_hip().linear_attention_step(
-        _unit(q), _unit(k), _unit(v), log_decay, state, out_state, done,
-        scale)
-    return out, out_state
+    with torch.no_grad():
+        out, new = _eager(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0),
+                          log_decay,
+                          None if done is None else done.unsqueeze(0),
+                          state, scale)
+        if out_state is not None:
+            new = out_state.copy_(new)
+    return out[0], new
