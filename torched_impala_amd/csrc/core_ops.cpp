@@ -664,6 +664,15 @@ long plan_product(ns::Args& a, int mode, int tile) {
   // least: below that, adding the parts costs more than it saves. Nothing is
   // split where the blocks fill the card anyway or the gain is small.
   long per = std::max((work + slots - 1) / slots, 512L / ks);
+  auto blocks_at = [&](long steps_a_block) {
+    long n = 0;
+    for (int i = 0; i < a.count; ++i)
+      n += a.mat[i].tiles *
+           (((mode == 0 ? a.mat[i].np : a.mat[i].mp) / ks + steps_a_block -
+             1) / steps_a_block);
+    return n;
+  };
+  while (per < longest && blocks_at(per) > slots) ++per;
   if (total >= slots || longest * 2 <= per * 3) per = longest;
   long part = 0;
   int blocks = 0, sums = 0;

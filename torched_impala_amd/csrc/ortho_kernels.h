@@ -5,7 +5,7 @@ namespace impala {
 namespace ortho {
 
 constexpr int MAX_MATS = 24;   // of one launch; all fit the kernel's arguments
-constexpr int MAX_NORM_BLOCKS = 256;   // of one matrix
+constexpr int MAX_NORM_BLOCKS = 1024;   // of one matrix
 
 // One matrix, worked on as m x n with m <= n (a tall one is turned), both
 // padded with zeros to whole tiles. Offsets are in elements of the workspace

@@ -52,10 +52,12 @@ __device__ inline void store_any(void* p, long i, int type, float v) {
   else ((half_t*)p)[i] = (half_t)v;
 }
 
+// the matrix that a block belongs to: all bounds compared at once (one after
+// the other each waits for a scalar load)
 __device__ inline int mat_of(const int* first, int count, int block) {
-  int i = 0;
-  while (i + 1 < count && block >= first[i + 1]) ++i;
-  return i;
+  const int l = threadIdx.x & 63;
+  const bool past = l + 1 < count && block >= first[l + 1 < count ? l + 1 : 0];
+  return __builtin_amdgcn_readfirstlane((int)__popcll(__ballot(past)));
 }
 
 // exponent of the power of two at or below the bound of |X| in round k
@@ -90,11 +92,39 @@ __global__ void __launch_bounds__(256) ns_norm(Args args) {
   const int fast = by_i ? M.m : M.n;
   const long sf = by_i ? M.src_i : M.src_j, ss = by_i ? M.src_j : M.src_i;
   double acc = 0.0;
-  if (sf == 1 && ss == fast) {   // dense: no division an element
-    #pragma unroll 4
-    for (long e = (long)blk * 256 + threadIdx.x; e < total; e += stride) {
-      const double v = load_any(M.src, e, M.type);
-      acc = fma(v, v, acc);
+  if (sf == 1 && ss == fast) {   // dense: no division, 16 bytes at a time
+    const int es = M.type == 0 ? 4 : 2, per = 16 / es;
+    const long head = ((16 - ((uintptr_t)M.src & 15)) & 15) / es;
+    const long lead = head < total ? head : total;
+    const long vecs = (total - lead) / per;
+    const char* base = (const char*)M.src + lead * es;
+    for (long e = (long)blk * 256 + threadIdx.x; e < vecs; e += stride) {
+      const u32x4 q = *reinterpret_cast<const u32x4*>(base + e * 16);
+      #pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned w = q[k];   // not cast in the vector: its first
+        if (M.type == 0) {         // element would be taken each time
+          const double v = __builtin_bit_cast(float, w);
+          acc = fma(v, v, acc);
+        } else {
+          #pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned short u = (unsigned short)(w >> (16 * h));
+            const double v = M.type == 1
+                ? (float)__builtin_bit_cast(bf16_t, u)
+                : (float)__builtin_bit_cast(half_t, u);
+            acc = fma(v, v, acc);
+          }
+        }
+      }
+    }
+    if (blk == 0) {   // what lies before and behind the 16-byte pieces
+      const long rest = total - vecs * per;
+      for (long e = threadIdx.x; e < rest; e += 256) {
+        const double v = load_any(M.src, e < lead ? e : e + vecs * per,
+                                  M.type);
+        acc = fma(v, v, acc);
+      }
     }
   } else {
     for (long e = (long)blk * 256 + threadIdx.x; e < total; e += stride) {
@@ -122,10 +152,10 @@ __global__ void __launch_bounds__(256) ns_prepare(Args args) {
   const int tn = M.np / 64;
   const int i0 = (t / tn) * 64, j0 = (t % tn) * 64;
 
-  static_assert(MAX_NORM_BLOCKS <= 256, "one partial sum a thread");
-  const double norm = sqrt(block_sum(
-      (int)threadIdx.x < M.norm_blocks
-          ? args.sums[args.first_norm[mi] + threadIdx.x] : 0.0));
+  double part = 0.0;
+  for (int k = threadIdx.x; k < M.norm_blocks; k += 256)
+    part += args.sums[args.first_norm[mi] + k];
+  const double norm = sqrt(block_sum(part));
   const float rho = (float)(norm / (norm + args.eps));
   const int e = M.ex - bound_exp(rho, 0);
   const double mul = ldexp(1.0 / (norm + args.eps), e);
