@@ -118,6 +118,12 @@ struct EngineBF16 {
     return __builtin_bit_cast(
         Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
+  static __device__ void store4(L* p, int part, f32x4 x) {
+    const bf16x4 h = __builtin_convertvector(x, bf16x4);
+    *reinterpret_cast<bf16x4*>(p) = h;
+    *reinterpret_cast<bf16x4*>(p + part) = __builtin_convertvector(
+        x - __builtin_convertvector(h, f32x4), bf16x4);
+  }
   static __device__ float at(const Frag& f, int e) { return (float)f[e]; }
   // fp32 values in N bf16 parts each, two at a time as the hardware converts
   template <int N>
@@ -133,13 +139,6 @@ struct EngineBF16 {
         if (n + 1 < N) x -= __builtin_convertvector(h, f32x2);
       }
     }
-  }
-  static __device__ void store4(L* p, int part, const float* v) {
-    const f32x4 x = {v[0], v[1], v[2], v[3]};
-    const bf16x4 h = __builtin_convertvector(x, bf16x4);
-    *reinterpret_cast<bf16x4*>(p) = h;
-    *reinterpret_cast<bf16x4*>(p + part) = __builtin_convertvector(
-        x - __builtin_convertvector(h, f32x4), bf16x4);
   }
 };
 
@@ -177,20 +176,34 @@ struct EngineF32 {
     }
     return f;
   }
+  static __device__ void store4(L* p, int, f32x4 x) {
+    *reinterpret_cast<f32x4*>(p) = x;
+  }
   static __device__ float at(const Frag& f, int e) { return f.x[e >> 2][e & 3]; }
   template <int N>
   static __device__ void split(const float* v, Frag* out) {
     #pragma unroll
     for (int e = 0; e < 8; ++e) out[0].x[e >> 2][e & 3] = v[e];
   }
-  static __device__ void store4(L* p, int, const float* v) {
-    f32x4 q = {v[0], v[1], v[2], v[3]};
-    *reinterpret_cast<f32x4*>(p) = q;
-  }
 };
 
 template <typename T> struct EngineOf { typedef EngineF32 E; };
 template <> struct EngineOf<bf16_t> { typedef EngineBF16 E; };
+
+// How a workgroup divides its work: NV blocks of 16 value columns a wave, and
+// whether the waves share the blocks of P through LDS or each computes all of
+// them in registers. bf16, forward pass: heads of 64 (T=101, B=512, 4 heads)
+// 44 us with two and all, 47 with one and shared; heads of 128 (T=512, B=64,
+// 8 heads) 117 us with one and shared, 127 with two and shared, 123 with two
+// and all. fp32 products are slow enough to be worth sharing.
+template <typename T, int D> struct Split {
+  static constexpr int NV = 1;
+  static constexpr bool SHARE = true;
+};
+template <int D> struct Split<bf16_t, D> {
+  static constexpr int NV = D > 64 ? 1 : 2;
+  static constexpr bool SHARE = D > 64;
+};
 
 // --------------------------------------------------------------------------
 // One chunk's rows of one operand, in registers on the way to LDS. Loads take
@@ -198,9 +211,8 @@ template <> struct EngineOf<bf16_t> { typedef EngineBF16 E; };
 // cleared on the way out. (With a branch, the compiler merges its sides by
 // copies that wait for the loads on the spot.)
 // --------------------------------------------------------------------------
-template <typename T, int D, bool VEC>
+template <typename T, int D, int THREADS, bool VEC>
 struct Rows {
-  static constexpr int THREADS = 4 * D;
   static constexpr int V = 16 / sizeof(T);
   static constexpr int PER_ROW = D / V;
   static constexpr int STEP = THREADS / PER_ROW;   // rows between pieces
@@ -265,41 +277,38 @@ struct Rows {
   }
 };
 
-// waves that a SIMD holds: as many as the LDS of a CU leaves room for, which
-// sets how many registers a wave may take
-template <typename T, int D>
-constexpr int waves_per_simd() {
-  return sizeof(typename EngineOf<T>::E::L) == 4 ? 2
-         : D == 64 || D == 96 ? 3 : 2;
-}
-
 // --------------------------------------------------------------------------
-// T: type of the operands. D: head size as it is padded, 32 to 128; D / 16
-// waves. VEC: 16-byte loads. STATE_ONLY: the first pass of cut sequences,
-// which leaves a segment's own state and has no rows of a result.
+// T: type of the operands. D: head size as it is padded, 32 to 128. VEC:
+// 16-byte loads. STATE_ONLY: the first pass of cut sequences, which leaves a
+// segment's own state and has no rows of a result.
 //
 // Nothing inside a chunk branches on its length: rows and columns beyond the
 // real ones are zeros in LDS and cost less than the waits between the basic
-// blocks that a test of every 16 x 16 block makes (measured on one chunk of
-// fp32, 64 wide: 6 us with the tests, see below without).
+// blocks that a test of every 16 x 16 block makes.
 // --------------------------------------------------------------------------
+template <typename T, int D>
+constexpr int threads_of() { return 4 * D / Split<T, D>::NV; }
+
 template <typename T, int D, bool VEC, bool STATE_ONLY>
-__global__ void __launch_bounds__(4 * D, (waves_per_simd<T, D>()))
+__global__ void __launch_bounds__((threads_of<T, D>()), 2)
 attn_chunks(AttnArgs args) {
   typedef typename EngineOf<T>::E E;
   typedef typename E::L L;
   typedef typename E::Frag Frag;
-  constexpr int THREADS = 4 * D;
-  constexpr int NW = D / 16;      // waves
+  constexpr int THREADS = threads_of<T, D>();
+  constexpr int NW = THREADS / 64;   // waves
+  constexpr int NV = Split<T, D>::NV;   // 16-column blocks of a wave's values
+  constexpr int NT = D / 16;         // 16-row blocks of the state's first axis
+  constexpr int NS = D / 32;         // products over 32 of that axis
   constexpr int LD = D + E::PAD;
   constexpr int LDP = C + E::PAD;
-  constexpr int NT = D / 16;      // 16-row blocks of the state's first axis
+  constexpr bool SHARE = Split<T, D>::SHARE && !STATE_ONLY;
   constexpr int PART = C * LDP;
 
   __shared__ __align__(16) L sa[STATE_ONLY ? 1 : C * LD];
   __shared__ __align__(16) L sb[C * LD];
   __shared__ __align__(16) L sc[C * LD];
-  __shared__ __align__(16) L sp[STATE_ONLY ? 8 : E::NP * PART];
+  __shared__ __align__(16) L sp[SHARE ? E::NP * PART : 8];
   __shared__ float pw[C + 1];
   __shared__ __align__(16) float w_out[C];
   __shared__ float w_in[C];
@@ -348,66 +357,90 @@ attn_chunks(AttnArgs args) {
                : reinterpret_cast<const unsigned char*>(args.log_decay);
   const long done_st = has_done ? args.done_st : 0;
 
-  Rows<T, D, VEC> ra, rb, rc;
+  Rows<T, D, THREADS, VEC> ra, rb, rc;
   unsigned dn = 0;   // as loaded: a test here would wait for all loads
-  // chunk n in the order of travel: its lowest step
-  auto chunk_at = [&](int n) __attribute__((always_inline)) {
-    return t_lo + (long)(rev ? chunks - 1 - n : n) * C;
-  };
+  // Chunks in the order of travel, each by its lowest step. Where the next
+  // one lies is carried along: the strides stay in few scalar registers.
+  const int tail = (int)(t_hi - t_lo - (long)(chunks - 1) * C);
+  const int tail_at = rev ? 0 : chunks - 1;
+  long t_next = t_lo + (rev ? (long)(chunks - 1) * C : 0);
+  const long dir = rev ? -C : C;
+  const T* na = pa + t_next * R.a.st;
+  const T* nb = pb + t_next * R.b.st;
+  const T* nc = pc + t_next * R.c.st;
+  const unsigned char* nd = pd + t_next * done_st;
+  const long sta = R.a.st, stb = R.b.st, stc = R.c.st;
   // behind the last chunk one row of it is read again and not used
   auto fetch = [&](int n) __attribute__((always_inline)) {
-    const bool real = n < chunks;
-    const long t0 = chunk_at(real ? n : chunks - 1);
-    const int len = !real ? 1 : (int)(t_hi - t0 < C ? t_hi - t0 : C);
-    dn = pd[(t0 + (l < len ? l : len - 1)) * done_st];
-    if constexpr (!STATE_ONLY)
-      ra.load(pa + t0 * R.a.st, R.a.st, len, dk, rev);
-    rb.load(pb + t0 * R.b.st, R.b.st, len, dk, rev);
-    rc.load(pc + t0 * R.c.st, R.c.st, len, dv, rev);
+    const int len = n >= chunks ? 1 : n == tail_at ? tail : C;
+    dn = nd[(l < len ? l : len - 1) * (int)done_st];
+    if constexpr (!STATE_ONLY) ra.load(na, sta, len, dk, rev);
+    rb.load(nb, stb, len, dk, rev);
+    rc.load(nc, stc, len, dv, rev);
+    if (n + 1 < chunks) {
+      na += dir * sta;
+      nb += dir * stb;
+      nc += dir * stc;
+      nd += dir * done_st;
+    }
   };
   fetch(0);
 
-  // the wave's part of S: block t, column y, rows 16 t + 4 g + r
-  f32x4 S[NT];
-  const int y = 16 * wave + m;
+  // the wave's part of S: block t, column y0 + 16 v, rows 16 t + 4 g + r
+  f32x4 S[NT][NV];
+  const int y0 = 16 * NV * wave + m;
   const bool whole = dk == D && dv == D;
   const long s_size = (long)dk * dv;
   bool any_state = R.s_in != nullptr;
   #pragma unroll
-  for (int t = 0; t < NT; ++t) S[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < NT; ++t) {
+    #pragma unroll
+    for (int v = 0; v < NV; ++v) S[t][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
   if (any_state) {
     const float* q = R.s_in + ((long)seg * heads + bh) * s_size;
     const int sx = (int)R.sx, sy = (int)R.sy;
     if (whole) {
-      const unsigned at = 4 * g * sx + y * sy;
+      const unsigned at = 4 * g * sx + y0 * sy;
       #pragma unroll
       for (int t = 0; t < NT; ++t) {
         #pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][r] = (q + (16 * t + r) * sx)[at];
+        for (int v = 0; v < NV; ++v) {
+          #pragma unroll
+          for (int r = 0; r < 4; ++r)
+            S[t][v][r] = (q + (16 * t + r) * sx + 16 * v * sy)[at];
+        }
       }
     } else {   // from clamped places, all at once, and cleared beyond the size
-      q += (y < dv ? y : dv - 1) * sy;
       #pragma unroll
       for (int t = 0; t < NT; ++t) {
         #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int x = 16 * t + 4 * g + r;
-          S[t][r] = q[(x < dk ? x : dk - 1) * sx];
+        for (int v = 0; v < NV; ++v) {
+          const int y = y0 + 16 * v;
+          #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int x = 16 * t + 4 * g + r;
+            S[t][v][r] = q[(x < dk ? x : dk - 1) * sx +
+                           (y < dv ? y : dv - 1) * sy];
+          }
         }
       }
       #pragma unroll
       for (int t = 0; t < NT; ++t) {
         #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * t + 4 * g + r >= dk || y >= dv) S[t][r] = 0.f;
+        for (int v = 0; v < NV; ++v) {
+          #pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * t + 4 * g + r >= dk || y0 + 16 * v >= dv)
+              S[t][v][r] = 0.f;
+        }
       }
     }
   }
 
   const Decay decay(args.log_decay[h * args.g_stride]);
   for (int i = tid; i <= C; i += THREADS) pw[i] = decay.pow((float)i);
-  if constexpr (!STATE_ONLY) {
-    // blocks of P that the mask leaves out stay zero
+  if constexpr (SHARE) {   // blocks of P that the mask leaves out stay zero
     u32x4* z = reinterpret_cast<u32x4*>(sp);
     constexpr int NZ = E::NP * PART * (int)sizeof(L) / 16;
     for (int i = tid; i < NZ; i += THREADS) z[i] = u32x4{0, 0, 0, 0};
@@ -415,18 +448,24 @@ attn_chunks(AttnArgs args) {
   bool seen_done = false;
   __syncthreads();
 
-  // the wave's blocks of P (ten on and under the diagonal, over the waves)
-  // and e^{g (i - j)} at the lane's places in them, 0 above the diagonal
-  constexpr int NP = (10 + NW - 1) / NW;
+  // Blocks of P on and under the diagonal: with SHARE the wave's own of the
+  // ten, else the four distances from it. e^{g (i - j)} at the lane's places
+  // in them, 0 above the diagonal
+  constexpr int NP = SHARE ? (10 + NW - 1) / NW : 4;
   float wt[NP][4];
   int p_it[NP], p_jt[NP];
   if constexpr (!STATE_ONLY) {
     #pragma unroll
     for (int e = 0; e < NP; ++e) {
-      // a wave without a block of its own computes the last one too
-      const int k = wave + NW * e < 10 ? wave + NW * e : 9;
-      p_it[e] = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0;
-      p_jt[e] = k - p_it[e] * (p_it[e] + 1) / 2;
+      if constexpr (SHARE) {
+        // a wave without a block of its own computes the last one too
+        const int k = wave + NW * e < 10 ? wave + NW * e : 9;
+        p_it[e] = k >= 6 ? 3 : k >= 3 ? 2 : k >= 1 ? 1 : 0;
+        p_jt[e] = k - p_it[e] * (p_it[e] + 1) / 2;
+      } else {
+        p_it[e] = e;
+        p_jt[e] = 0;
+      }
       #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int lag = 16 * (p_it[e] - p_jt[e]) + m - 4 * g - r;
@@ -435,11 +474,12 @@ attn_chunks(AttnArgs args) {
     }
   }
   // this wave has columns of the result
-  const bool idle = 16 * wave >= dv;
+  const bool idle = 16 * NV * wave >= dv;
 
   for (int n = 0; n < chunks; ++n) {
-    const long t0 = chunk_at(n);
-    const int len = (int)(t_hi - t0 < C ? t_hi - t0 : C);
+    const long t0 = t_next;
+    const int len = n == tail_at ? tail : C;
+    t_next += dir;
 
     // ---- stage: rows to LDS, weights of the chunk's rows
     if constexpr (!STATE_ONLY) ra.store(sa, LD, len, dk);
@@ -470,93 +510,158 @@ attn_chunks(AttnArgs args) {
     fetch(n + 1);
 
     bool finite = true;
-    if constexpr (!STATE_ONLY) {
+    if constexpr (SHARE) {
       // ---- P, transposed in the products (a result's column is row i, its
-      // rows are j), ten blocks over the waves
+      // rows are j)
       f32x4 acc[NP];
       #pragma unroll
       for (int e = 0; e < NP; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
       #pragma unroll
-      for (int s = 0; s < D / 32; ++s) {
+      for (int s = 0; s < NS; ++s) {
         #pragma unroll
         for (int e = 0; e < NP; ++e)
           acc[e] = E::mma(E::rows(sb, LD, 16 * p_jt[e], 32 * s, l),
                           E::rows(sa, LD, 16 * p_it[e], 32 * s, l), acc[e]);
       }
-      float p[NP][4];
       #pragma unroll
       for (int e = 0; e < NP; ++e) {
         #pragma unroll
-        for (int r = 0; r < 4; ++r) p[e][r] = acc[e][r] * wt[e][r];
+        for (int r = 0; r < 4; ++r) acc[e][r] *= wt[e][r];
       }
       if (any_cut) {
+        asm volatile("");   // a branch: most chunks have no cut
         #pragma unroll
         for (int e = 0; e < NP; ++e) {
           const int lo = first[16 * p_it[e] + m] - 16 * p_jt[e] - 4 * g;
           #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (r < lo) p[e][r] = 0.f;
+            if (r < lo) acc[e][r] = 0.f;
         }
       }
       #pragma unroll
       for (int e = 0; e < NP; ++e)
         E::store4(sp + (16 * p_it[e] + m) * LDP + 16 * p_jt[e] + 4 * g, PART,
-                  p[e]);
+                  acc[e]);
     }
 
-    f32x4 O[4];
-    Frag cf[2];
+    f32x4 O[4][NV];
+    Frag cf[2][NV];
     if (!idle) {
       if constexpr (!STATE_ONLY) {
         // ---- what came before the chunk: a S, weighted per row
         #pragma unroll
-        for (int it = 0; it < 4; ++it) O[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int it = 0; it < 4; ++it) {
+          #pragma unroll
+          for (int v = 0; v < NV; ++v) O[it][v] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
         if (any_state) {
           #pragma unroll
-          for (int s = 0; s < D / 32; ++s) {
-            Frag sf[E::NP];
-            float x[8];
+          for (int s = 0; s < NS; ++s) {
+            Frag sf[NV][E::NP];
             #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              x[r] = S[2 * s][r];
-              x[4 + r] = S[2 * s + 1][r];
+            for (int v = 0; v < NV; ++v) {
+              float x[8];
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                x[r] = S[2 * s][v][r];
+                x[4 + r] = S[2 * s + 1][v][r];
+              }
+              E::template split<E::NP>(x, sf[v]);
             }
-            E::template split<E::NP>(x, sf);
             #pragma unroll
             for (int it = 0; it < 4; ++it) {
               const Frag af = E::rows(sa, LD, 16 * it, 32 * s, l);
               #pragma unroll
-              for (int p = 0; p < E::NP; ++p)
-                O[it] = E::mma(sf[p], af, O[it]);
+              for (int p = 0; p < E::NP; ++p) {
+                #pragma unroll
+                for (int v = 0; v < NV; ++v)
+                  O[it][v] = E::mma(sf[v][p], af, O[it][v]);
+              }
             }
           }
           #pragma unroll
           for (int it = 0; it < 4; ++it) {
             const float w = w_in[16 * it + m];
             #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              O[it][r] *= w;
+            for (int v = 0; v < NV; ++v) {
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) O[it][v][r] *= w;
+            }
           }
         }
       }
       // ---- c, as it is needed twice: left operand here, right one below
       #pragma unroll
-      for (int s = 0; s < 2; ++s)
-        cf[s] = E::cols(sc, LD, 32 * s, 16 * wave, l);
+      for (int s = 0; s < 2; ++s) {
+        #pragma unroll
+        for (int v = 0; v < NV; ++v)
+          cf[s][v] = E::cols(sc, LD, 32 * s, 16 * (NV * wave + v), l);
+      }
     }
-    if constexpr (!STATE_ONLY) __syncthreads();   // P is whole
+    if constexpr (SHARE) __syncthreads();   // P is whole
     if (!idle) {
       if constexpr (!STATE_ONLY) {
         // row blocks 0 and 1 meet the first 32 rows of j, 2 and 3 all
         #pragma unroll
         for (int it = 0; it < 4; ++it) {
-          #pragma unroll
-          for (int s = 0; s <= it >> 1; ++s) {
+          if constexpr (SHARE) {
             #pragma unroll
-            for (int p = 0; p < E::NP; ++p)
-              O[it] = E::mma(cf[s],
-                             E::rows(sp + p * PART, LDP, 16 * it, 32 * s, l),
-                             O[it]);
+            for (int s = 0; s <= it >> 1; ++s) {
+              #pragma unroll
+              for (int p = 0; p < E::NP; ++p) {
+                const Frag pf =
+                    E::rows(sp + p * PART, LDP, 16 * it, 32 * s, l);
+                #pragma unroll
+                for (int v = 0; v < NV; ++v)
+                  O[it][v] = E::mma(cf[s][v], pf, O[it][v]);
+              }
+            }
+          } else {
+            // ---- the row block of P, transposed in the products, so that
+            // it comes out as the right operand of the next one
+            f32x4 acc[4];
+            #pragma unroll
+            for (int jt = 0; jt < 4; ++jt) acc[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+            #pragma unroll
+            for (int s = 0; s < NS; ++s) {
+              const Frag af = E::rows(sa, LD, 16 * it, 32 * s, l);
+              #pragma unroll
+              for (int jt = 0; jt <= it; ++jt)
+                acc[jt] = E::mma(E::rows(sb, LD, 16 * jt, 32 * s, l), af,
+                                 acc[jt]);
+            }
+            #pragma unroll
+            for (int jt = 0; jt <= it; ++jt) {
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) acc[jt][r] *= wt[it - jt][r];
+            }
+            if (any_cut) {
+              asm volatile("");   // a branch: most chunks have no cut
+              const int lo = first[16 * it + m] - 4 * g;
+              #pragma unroll
+              for (int jt = 0; jt <= it; ++jt) {
+                #pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (16 * jt + r < lo) acc[jt][r] = 0.f;
+              }
+            }
+            #pragma unroll
+            for (int s = 0; s <= it >> 1; ++s) {
+              float x[8];
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                x[r] = acc[2 * s][r];
+                x[4 + r] = acc[2 * s + 1][r];
+              }
+              Frag pf[E::NP];
+              E::template split<E::NP>(x, pf);
+              #pragma unroll
+              for (int p = 0; p < E::NP; ++p) {
+                #pragma unroll
+                for (int v = 0; v < NV; ++v)
+                  O[it][v] = E::mma(cf[s][v], pf[p], O[it][v]);
+              }
+            }
           }
         }
         // An input that is not finite always shows in the row that it
@@ -566,22 +671,29 @@ attn_chunks(AttnArgs args) {
         #pragma unroll
         for (int it = 0; it < 4; ++it) {
           #pragma unroll
-          for (int r = 0; r < 4; ++r) z[r] = fmaf(O[it][r], 0.f, z[r]);
+          for (int v = 0; v < NV; ++v) {
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) z[r] = fmaf(O[it][v][r], 0.f, z[r]);
+          }
         }
         finite = !__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f);
         if (finite) {
-          const int x0 = 16 * wave + 4 * g;
+          const int x0 = 16 * NV * wave + 4 * g;
           if constexpr (VEC) {   // dv is a multiple of 4, 64 rows in 32 bits
             T* q = po + (rev ? t0 + len - C : t0) * so;
             const long step = (rev ? -16 : 16) * so;
             const unsigned at = (unsigned)((rev ? C - 1 - m : m) * so + x0);
             #pragma unroll
             for (int it = 0; it < 4; ++it) {
-              struct alignas(4 * sizeof(T)) { T e[4]; } w;
               #pragma unroll
-              for (int r = 0; r < 4; ++r) w.e[r] = (T)O[it][r];
-              if (16 * it + m < len && x0 < dv)
-                *reinterpret_cast<decltype(w)*>(q + it * step + at) = w;
+              for (int v = 0; v < NV; ++v) {
+                struct alignas(4 * sizeof(T)) { T e[4]; } w;
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) w.e[r] = (T)O[it][v][r];
+                if (16 * it + m < len && x0 + 16 * v < dv)
+                  *reinterpret_cast<decltype(w)*>(q + it * step + 16 * v +
+                                                  at) = w;
+              }
             }
           } else {
             #pragma unroll
@@ -589,41 +701,51 @@ attn_chunks(AttnArgs args) {
               const int i = 16 * it + m;
               T* q = po + (t0 + (rev ? len - 1 - i : i)) * so + x0;
               #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (i < len && x0 + r < dv) q[r] = (T)O[it][r];
+              for (int v = 0; v < NV; ++v) {
+                #pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (i < len && x0 + 16 * v + r < dv)
+                    q[16 * v + r] = (T)O[it][v][r];
+              }
             }
           }
         }
       }
       // ---- the state behind the chunk
       if (finite) {
-        Frag cw[2][E::NU];
+        f32x4 U[NT][NV];
+        #pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          #pragma unroll
+          for (int v = 0; v < NV; ++v) {
+            #pragma unroll
+            for (int r = 0; r < 4; ++r) U[t][v][r] = S[t][v][r] * keep;
+          }
+        }
         #pragma unroll
         for (int s = 0; s < 2; ++s) {
           const f32x4 w0 = *reinterpret_cast<const f32x4*>(
               w_out + 32 * s + 4 * g);
           const f32x4 w1 = *reinterpret_cast<const f32x4*>(
               w_out + 32 * s + 16 + 4 * g);
-          float x[8];
+          Frag cw[NV][E::NU];
           #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            x[e] = E::at(cf[s], e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
+          for (int v = 0; v < NV; ++v) {
+            float x[8];
+            #pragma unroll
+            for (int e = 0; e < 8; ++e)
+              x[e] = E::at(cf[s][v], e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
+            E::template split<E::NU>(x, cw[v]);
           }
-          E::template split<E::NU>(x, cw[s]);
-        }
-        f32x4 U[NT];
-        #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          #pragma unroll
-          for (int r = 0; r < 4; ++r) U[t][r] = S[t][r] * keep;
-        }
-        #pragma unroll
-        for (int s = 0; s < 2; ++s) {
           #pragma unroll
           for (int t = 0; t < NT; ++t) {
             const Frag bf = E::cols(sb, LD, 32 * s, 16 * t, l);
             #pragma unroll
-            for (int p = 0; p < E::NU; ++p) U[t] = E::mma(bf, cw[s][p], U[t]);
+            for (int p = 0; p < E::NU; ++p) {
+              #pragma unroll
+              for (int v = 0; v < NV; ++v)
+                U[t][v] = E::mma(bf, cw[v][p], U[t][v]);
+            }
           }
         }
         if constexpr (STATE_ONLY) {   // no rows that would show it
@@ -631,50 +753,64 @@ attn_chunks(AttnArgs args) {
           #pragma unroll
           for (int t = 0; t < NT; ++t) {
             #pragma unroll
-            for (int r = 0; r < 4; ++r) z[r] = fmaf(U[t][r], 0.f, z[r]);
+            for (int v = 0; v < NV; ++v) {
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) z[r] = fmaf(U[t][v][r], 0.f, z[r]);
+            }
           }
           finite = !__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f);
         }
         if (finite) {
           #pragma unroll
-          for (int t = 0; t < NT; ++t) S[t] = U[t];
+          for (int t = 0; t < NT; ++t) {
+            #pragma unroll
+            for (int v = 0; v < NV; ++v) S[t][v] = U[t][v];
+          }
         }
       }
       // ---- step by step, where something is not finite
       if (!finite) {
-        for (int i = 0; i < len; ++i) {
-          // what lies before the first row backwards has not decayed
-          const bool cut = (cuts >> i) & 1;
-          const float f = rev && i == 0 ? 1.f : pw[1];
-          const float cy = (float)sc[i * LD + y] * R.u_scale;
-          float o = 0.f;
-          #pragma unroll
-          for (int t = 0; t < NT; ++t) {
+        // sizes that the compiler cannot take for those outside: it would
+        // compute the masks below in front of the loop, for every chunk
+        int dk_ = dk, dv_ = dv;
+        asm volatile("" : "+s"(dk_), "+s"(dv_));
+        #pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int y = y0 + 16 * v;
+          for (int i = 0; i < len; ++i) {
+            // what lies before the first row backwards has not decayed
+            const bool cut = (cuts >> i) & 1;
+            const float f = rev && i == 0 ? 1.f : pw[1];
+            const float cy = (float)sc[i * LD + y] * R.u_scale;
+            float o = 0.f;
             #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const int x = 16 * t + 4 * g + r;
-              if (x < dk && y < dv) {
-                S[t][r] = fmaf((float)sb[i * LD + x], cy,
-                               cut ? 0.f : S[t][r] * f);
-                if constexpr (!STATE_ONLY)
-                  o = fmaf((float)sa[i * LD + x], S[t][r], o);
+            for (int t = 0; t < NT; ++t) {
+              #pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                const int x = 16 * t + 4 * g + r;
+                if (x < dk_ && y < dv_) {
+                  S[t][v][r] = fmaf((float)sb[i * LD + x], cy,
+                                    cut ? 0.f : S[t][v][r] * f);
+                  if constexpr (!STATE_ONLY)
+                    o = fmaf((float)sa[i * LD + x], S[t][v][r], o);
+                }
               }
             }
+            if constexpr (!STATE_ONLY) {
+              o += __shfl_xor(o, 16, 64);
+              o += __shfl_xor(o, 32, 64);
+              if (g == 0 && y < dv_)
+                po[(t0 + (rev ? len - 1 - i : i)) * so + y] =
+                    (T)(o * R.in_scale);
+            }
           }
-          if constexpr (!STATE_ONLY) {
-            o += __shfl_xor(o, 16, 64);
-            o += __shfl_xor(o, 32, 64);
-            if (g == 0 && y < dv)
-              po[(t0 + (rev ? len - 1 - i : i)) * so + y] =
-                  (T)(o * R.in_scale);
-          }
-        }
-        if (rev) {
-          #pragma unroll
-          for (int t = 0; t < NT; ++t) {
+          if (rev) {
             #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              S[t][r] = cut_behind ? 0.f : S[t][r] * pw[1];
+            for (int t = 0; t < NT; ++t) {
+              #pragma unroll
+              for (int r = 0; r < 4; ++r)
+                S[t][v][r] = cut_behind ? 0.f : S[t][v][r] * pw[1];
+            }
           }
         }
       }
@@ -693,19 +829,27 @@ attn_chunks(AttnArgs args) {
     float* q = R.s_out + (STATE_ONLY ? (long)seg * heads + bh : (long)bh) *
                              s_size;
     if (whole) {
-      const unsigned at = 4 * g * D + y;
+      const unsigned at = 4 * g * D + y0;
       #pragma unroll
       for (int t = 0; t < NT; ++t) {
         #pragma unroll
-        for (int r = 0; r < 4; ++r) (q + (16 * t + r) * D)[at] = S[t][r];
+        for (int v = 0; v < NV; ++v) {
+          #pragma unroll
+          for (int r = 0; r < 4; ++r)
+            (q + (16 * t + r) * D + 16 * v)[at] = S[t][v][r];
+        }
       }
     } else {
       #pragma unroll
       for (int t = 0; t < NT; ++t) {
         #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int x = 16 * t + 4 * g + r;
-          if (x < dk && y < dv) q[x * dv + y] = S[t][r];
+        for (int v = 0; v < NV; ++v) {
+          const int y = y0 + 16 * v;
+          #pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int x = 16 * t + 4 * g + r;
+            if (x < dk && y < dv) q[x * dv + y] = S[t][v][r];
+          }
         }
       }
     }
@@ -722,12 +866,25 @@ attn_scan(float* __restrict__ st, const float* __restrict__ keep,
   if (i >= heads * size) return;
   const long bh = i / size;
   float run = first ? first[i] : 0.f;
-  for (int n = 0; n < nseg; ++n) {
-    const long s = rev ? nseg - 1 - n : n;
-    float* p = st + s * heads * size + i;
-    const float own = *p, k = keep[s * heads + bh];
-    *p = run;
-    run = (k == 0.f ? 0.f : run * k) + own;
+  // eight segments are read before the first is written: a load does not move
+  // over a store to the same array by itself
+  for (int n0 = 0; n0 < nseg; n0 += 8) {
+    float own[8], k[8];
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int n = n0 + e < nseg ? n0 + e : nseg - 1;
+      const long s = rev ? nseg - 1 - n : n;
+      own[e] = st[s * heads * size + i];
+      k[e] = keep[s * heads + bh];
+    }
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (n0 + e < nseg) {
+        const long s = rev ? nseg - 1 - n0 - e : n0 + e;
+        st[s * heads * size + i] = run;
+        run = (k[e] == 0.f ? 0.f : run * k[e]) + own[e];
+      }
+    }
   }
 }
 
@@ -828,11 +985,11 @@ template <typename T, int D, bool VEC>
 void run(const AttnArgs& a, bool state_only, hipStream_t s) {
   const dim3 grid((unsigned)((long)a.B * a.H * a.nseg * a.nroles));
   if (state_only)
-    hipLaunchKernelGGL((attn_chunks<T, D, VEC, true>), grid, dim3(4 * D), 0,
-                       s, a);
+    hipLaunchKernelGGL((attn_chunks<T, D, VEC, true>), grid,
+                       dim3(threads_of<T, D>()), 0, s, a);
   else
-    hipLaunchKernelGGL((attn_chunks<T, D, VEC, false>), grid, dim3(4 * D), 0,
-                       s, a);
+    hipLaunchKernelGGL((attn_chunks<T, D, VEC, false>), grid,
+                       dim3(threads_of<T, D>()), 0, s, a);
 }
 
 template <typename T, bool VEC>

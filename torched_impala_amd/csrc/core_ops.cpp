@@ -329,26 +329,38 @@ bool can_vec(const Tensor& t, const AttnOperand& o) {
          (t.size(-1) * es) % 16 == 0;
 }
 
-// segments that a sequence is cut into: none while the heads alone give the
-// card two workgroups a CU, else as many as make that up, four chunks each
-// at least (a segment's state costs as much traffic as some chunks do)
-int attn_segments(const AttnShape& s, long* seg_len) {
+// Segments that a sequence is cut into. Workgroups that run at once: what a
+// CU holds of the kernel's tiles (one of those for heads above 64, whose LDS
+// or registers fill it, two in fp32, four in bf16), times 256. Heads that
+// fill those by themselves are not cut. Else n segments take about
+// chunks / n * 9 us for their two passes and n states of all heads, moved five
+// times at 4 MB a us; the sum is least at the root below.
+int attn_segments(const AttnShape& s, int type, long* seg_len) {
   const long chunks = (s.T + 63) / 64, heads = s.B * s.H;
-  long n = heads >= 512 ? 1 : 512 / heads;
-  const long most = chunks / 4;
-  if (n > most) n = most;
+  const long slots = std::max(s.dk, s.dv) > 64 ? 256 : type == 1 ? 1024 : 512;
+  const double best = std::sqrt(chunks * 9.0 * 4e6 /
+                                (20.0 * heads * s.dk * s.dv));
+  long n = std::min({slots / heads, chunks, (long)std::min(best, 1e6)});
   if (n < 1) n = 1;
   const long per = (chunks + n - 1) / n;
   *seg_len = per * 64;
   return (int)((s.T + *seg_len - 1) / *seg_len);
 }
 
-AttnArgs attn_args(const AttnShape& s, const Tensor& g,
+// flags whose 64 steps lie within 32 bits
+Tensor near(const Tensor& done) {
+  return done.defined() && done.size(0) > 1 && done.stride(0) >= (1L << 25)
+             ? done.contiguous() : done;
+}
+
+AttnArgs attn_args(const AttnShape& s, int type, const Tensor& g,
                    const Tensor& done) {
   AttnArgs a{};
   a.log_decay = g.data_ptr<float>();
   a.g_stride = g.size(0) > 1 ? g.stride(0) : 0;
   if (done.defined()) {
+    TORCH_CHECK(done.size(0) == 1 || done.stride(0) < (1L << 25),
+                "linear_attention: steps of done lie too far apart");
     a.done = (const unsigned char*)done.data_ptr();
     a.done_st = done.size(0) > 1 ? done.stride(0) : 0;
     a.done_sb = done.size(1) > 1 ? done.stride(1) : 0;
@@ -356,7 +368,7 @@ AttnArgs attn_args(const AttnShape& s, const Tensor& g,
   a.T = s.T;
   a.B = (int)s.B;
   a.H = (int)s.H;
-  a.nseg = attn_segments(s, &a.seg_len);
+  a.nseg = attn_segments(s, type, &a.seg_len);
   TORCH_CHECK(s.B * s.H * a.nseg <= MAX_GRID / 3 &&
                   s.B * s.H * s.dk * s.dv / 256 < MAX_GRID,
               "linear_attention: batch too large");
@@ -389,12 +401,12 @@ AttnShape shape_of(const Tensor& q, const Tensor& v) {
 // (out, final state, entry states of segments or none)
 std::array<Tensor, 3> attn_fwd(const Tensor& q0, const Tensor& k0,
                                const Tensor& v0, const Tensor& g,
-                               const Tensor& done, const Tensor& state0,
+                               const Tensor& done0, const Tensor& state0,
                                double scale) {
   const AttnShape s = shape_of(q0, v0);
   const c10::DeviceGuard guard(q0.device());
   const Tensor q = unit(q0), k = unit(k0), v = unit(v0),
-               state = dense(state0);
+               state = dense(state0), done = near(done0);
   const int type = type_code(q, "q");
   Tensor out = torch::empty({s.T, s.B, s.H, s.dv}, q.options());
   Tensor fin = torch::empty({s.B, s.H, s.dk, s.dv},
@@ -406,7 +418,7 @@ std::array<Tensor, 3> attn_fwd(const Tensor& q0, const Tensor& k0,
     else fin.zero_();
     return {out, fin, entry};
   }
-  AttnArgs a = attn_args(s, g, done);
+  AttnArgs a = attn_args(s, type, g, done);
   AttnRole r{};
   r.a = operand(q, 2);
   r.b = operand(k, 2);
@@ -456,8 +468,8 @@ class LinearAttention : public torch::autograd::Function<LinearAttention> {
     const AttnShape s = shape_of(saved[0], saved[2]);
     const c10::DeviceGuard guard(saved[0].device());
     const Tensor q = unit(saved[0]), k = unit(saved[1]), v = unit(saved[2]);
-    const Tensor &g = saved[3], &done = saved[4], &entry = saved[6];
-    const Tensor state = dense(saved[5]);
+    const Tensor &g = saved[3], &entry = saved[6];
+    const Tensor done = near(saved[4]), state = dense(saved[5]);
     const Tensor d_out = grads[0].defined()
                              ? unit(grads[0])
                              : torch::zeros(v.sizes(), v.options());
@@ -471,7 +483,7 @@ class LinearAttention : public torch::autograd::Function<LinearAttention> {
       ds = torch::empty({s.B, s.H, s.dk, s.dv},
                         q.options().dtype(torch::kFloat32));
     if (s.B * s.H > 0 && s.T > 0) {
-      AttnArgs a = attn_args(s, g, done);
+      AttnArgs a = attn_args(s, type, g, done);
       const AttnOperand oq = operand(q, 2), ok = operand(k, 2),
                         ov = operand(v, 2), od = operand(d_out, 2);
       const bool vec = can_vec(q, oq) && can_vec(k, ok) && can_vec(v, ov) &&
