@@ -314,3 +314,13 @@ def test_saved_input_changed_in_place():
     z.add_(1.0)
     with pytest.raises(RuntimeError):
         y.sum().backward()
+
+
+@pytest.mark.gpu
+def test_differentiable_once():
+    x = torch.randn(4, 8, device="cuda", requires_grad=True)
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(layer_norm(x, w).square().sum(), x,
+                             create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

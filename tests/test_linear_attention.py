@@ -529,6 +529,54 @@ def test_saved_input_changed_in_place():
         out.sum().backward()
 
 
+@pytest.mark.gpu
+def test_differentiable_once():
+    q, k, v, g, d, s, do, df = _inputs(9, 1, 1, 8, 8, torch.float32)
+    q.requires_grad_()
+    out, _ = linear_attention(q, k, v, g, done=d, state=s)
+    gq, = torch.autograd.grad(out.square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gq.sum().backward()
+
+
+@pytest.mark.gpu
+def test_one_tensor_in_all_places():
+    _, _, _, g, d, s, do, df = _inputs(70, 2, 2, 16, 16, torch.float32)
+    x = torch.randn(70, 2, 2, 16, device="cuda")
+    a = x.clone().requires_grad_()
+    out, _ = linear_attention(a, a, a, g, done=d, state=s)
+    got, = torch.autograd.grad(out, a, do)
+    full = _run(x, x, x, g, d, s, do, None)
+    torch.testing.assert_close(got, full[2] + full[3] + full[4],
+                               rtol=1e-5, atol=1e-4)
+
+
+@pytest.mark.gpu
+def test_gradient_of_a_sum():
+    """The output's gradient comes as a broadcast view of one number."""
+    a = _inputs(70, 2, 2, 16, 16, torch.float32)
+    q, k, v, g, d, s, do, df = a
+    ins = [t.clone().requires_grad_() for t in (q, k, v)]
+    out, _ = linear_attention(*ins, g, done=d, state=s)
+    got = torch.autograd.grad(out.sum(), ins)
+    ref = _run(q, k, v, g, d, s, torch.ones_like(do), None)
+    for x, y in zip(got, ref[2:5]):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_flags_far_apart():
+    """Flags whose steps lie more than 2^25 bytes apart."""
+    T, far = 70, 2 ** 25 + 3
+    q, k, v, g, d, s, _, _ = _inputs(T, 1, 1, 8, 8, torch.float32)
+    base = torch.zeros(far * T, dtype=torch.bool, device="cuda")
+    d2 = base.as_strided((T, 1), (far, 1))
+    d2.copy_(d)
+    ref = linear_attention(q, k, v, g, done=d, state=s)
+    got = linear_attention(q, k, v, g, done=d2, state=s)
+    assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+
+
 # --------------------------------------------------------------- one step
 @pytest.mark.gpu
 @pytest.mark.parametrize("dk,dv", [(1, 1), (5, 3), (8, 4), (64, 64),

@@ -194,6 +194,11 @@ def test_trains_from_actors(tmp_path, optimizer):
     assert stats["step_frames"] == 4 * 10
 
 
+def test_eval_entry():
+    flags = Flags(env="cartpole", device="cpu", use_linear_attention=True)
+    assert len(L.test(flags, num_episodes=1)["returns"]) == 1
+
+
 # --------------------------------------------------------------- GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("T,B", [(1, 5), (21, 32), (101, 4), (700, 1)])
