@@ -38,6 +38,15 @@
 // every segment's own state, a scan over segments turns them into entry
 // states, and the segments then run side by side.
 //
+// Bound: for heads of 64 in bf16 mostly memory (T=101, B=512, 4 heads with a
+// state in and out: 44 us forward for 173 MB, which takes 31 us without any
+// arithmetic); for heads of 128 the chain of LDS reads and products inside a
+// chunk, with two waves a SIMD to hide it in (T=512, B=64, 8 heads: 116 us for
+// 335 MB; LDS 45 %, vector units 28 %, matrix units 19 % busy). Tried there
+// without gain: chunks of 32, four waves a SIMD (spills), two value blocks a
+// wave, rows 8 banks apart for the transposing reads, reads ordered ahead of
+// the products. fp32 is bound by its matrix rate, a sixteenth of bf16's.
+//
 // A product of masks lets NaN and infinities of the future or of an earlier
 // episode through (0 * inf). A chunk whose result is not finite is computed
 // again step by step, as the recurrence says, so that they reach exactly the
@@ -890,8 +899,10 @@ attn_scan(float* __restrict__ st, const float* __restrict__ keep,
 
 // --------------------------------------------------------------------------
 // one step: S' = e^g (1 - done) S + k v^T, o = scale q^T S'. Bound by reading
-// and writing the state once. A block owns a head: V columns a thread,
-// the rows in turns, the result added over the row groups in LDS.
+// and writing the state once: 103 us for 512 environments of 8 heads of
+// 128 x 128, 5.2 TB/s, as fast as a copy; 4.4 us for 32 of 4 heads of 64 x 64,
+// a launch. A block owns a head: V columns a thread, the rows in turns, the
+// result added over the row groups in LDS.
 // --------------------------------------------------------------------------
 template <typename T, int V>
 __global__ void __launch_bounds__(256)

@@ -6,7 +6,10 @@
 //   dw = sum over rows dy * xhat,     db = sum over rows dy
 //
 // Bound: memory. Forward has to read x and write y, backward to read x and
-// dy and write dx; everything else is per row or per column.
+// dy and write dx; everything else is per row or per column. Measured (copies
+// reach 5.15 TB/s on the same card): 16384 x 4096 bf16 forward 56 us (4.8
+// TB/s), backward 86 us (4.7 TB/s) and 7 us for the column sums; 51712 x 263
+// fp32 22, 32 and 4 us.
 //
 // A row lives in the registers of one group of threads, so x is read once
 // and the variance is the two-pass one (sum of squares around the mean, in
@@ -201,7 +204,7 @@ ln_bwd(const T* __restrict__ dy, const T* __restrict__ x, long xs,
     if (w && c < cols) load_vec<W, VEC>(w + c, &wv[i * VEC]);
   }
   // The next row is on its way while one is worked on: without that, a wave
-  // waits for memory once a row (108 -> 90 us for 16384 x 4096 bf16). Places
+  // waits for memory once a row (108 -> 86 us for 16384 x 4096 bf16). Places
   // beyond the rows and columns are clamped to real ones, so that the loads
   // take no branch, and left out of the sums.
   Raw<T, VEC> xr[NV], gr[NV];

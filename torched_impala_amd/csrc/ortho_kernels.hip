@@ -20,6 +20,11 @@
 // eps), times a each round, up to 1.25), so its entries are of the order of
 // beta_k / sqrt(n), and those of A of beta_k^2 / sqrt(m).
 //
+// Measured, a round of 2048 x 2048 and 2048 x 8192: 206 us for A, 112 for B,
+// 340 for X (0.76 PFLOP/s of fp16 products, where the library's large bf16
+// product reaches 1.05), 14 for adding parts. A round of the shallow net's
+// matrices (6, up to 1024 x 263 and 256 x 1568) takes 38 us, about 10 a launch.
+//
 // A and B are symmetric: only tiles on and under the diagonal are computed,
 // and written twice. X is kept in both orientations, so that every product
 // reads both operands along k.
