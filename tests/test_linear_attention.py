@@ -218,10 +218,32 @@ def test_refusals_cpu():
     _refuse("cpu")
 
 
+def _refuse_heads(device):
+    """More heads than a launch has threads for."""
+    from torched_impala_amd.ops.linear_attention import MAX_HEADS
+    x = torch.zeros(1, 1, 1, 1, device=device)
+    g = torch.zeros(3, device=device)
+    x = x.expand(1, MAX_HEADS // 3 + 1, 3, 1)
+    with pytest.raises(ValueError):
+        linear_attention(x, x, x, g)
+    with pytest.raises(ValueError):
+        linear_attention_step(x[0], x[0], x[0], g,
+                              x[0].unsqueeze(-1))
+
+
+def test_too_many_heads_cpu():
+    _refuse_heads("cpu")
+
+
 # --------------------------------------------------------------- GPU
 @pytest.mark.gpu
 def test_refusals_gpu():
     _refuse("cuda")
+
+
+@pytest.mark.gpu
+def test_too_many_heads_gpu():
+    _refuse_heads("cuda")
 
 
 LENGTHS = [1, 2, 15, 16, 17, 21, 33, 48, 63, 64, 65, 101, 128, 129, 200]

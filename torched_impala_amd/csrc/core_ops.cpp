@@ -235,7 +235,9 @@ using impala::attn::AttnRole;
 using impala::attn::AttnStepArgs;
 
 constexpr long MAX_HEAD = 128;   // the largest tile that the kernels have
-constexpr long MAX_GRID = 2147483647;
+// heads of a batch: a launch has at most 2^32 threads, 512 to a head in each
+// of three roles (a step's 256 are fewer)
+constexpr long MAX_HEADS = ((1L << 32) - 1) / (3 * 512);
 
 struct AttnShape {
   long T, B, H, dk, dv;
@@ -273,9 +275,8 @@ AttnShape check_attn(const char* op, const Tensor& q, const Tensor& k,
   TORCH_CHECK_VALUE(
       s.dk >= 1 && s.dk <= MAX_HEAD && s.dv >= 1 && s.dv <= MAX_HEAD, op,
       ": head sizes must be 1 to ", MAX_HEAD, ", not ", s.dk, " and ", s.dv);
-  TORCH_CHECK_VALUE(s.B <= MAX_GRID && s.H <= MAX_GRID &&
-                        s.B * s.H <= MAX_GRID / 3,
-                    op, ": batch too large");
+  TORCH_CHECK_VALUE(s.B == 0 || s.H <= MAX_HEADS / s.B, op,
+                    ": batch times heads must be at most ", MAX_HEADS);
   TORCH_CHECK_TYPE(g.scalar_type() == torch::kFloat32, op,
                    ": log_decay must be fp32, not ", g.scalar_type());
   TORCH_CHECK_VALUE(g.device() == q.device() && g.dim() == 1 &&
@@ -369,9 +370,6 @@ AttnArgs attn_args(const AttnShape& s, int type, const Tensor& g,
   a.B = (int)s.B;
   a.H = (int)s.H;
   a.nseg = attn_segments(s, type, &a.seg_len);
-  TORCH_CHECK(s.B * s.H * a.nseg <= MAX_GRID / 3 &&
-                  s.B * s.H * s.dk * s.dv / 256 < MAX_GRID,
-              "linear_attention: batch too large");
   return a;
 }
 

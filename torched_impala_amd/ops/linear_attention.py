@@ -23,6 +23,7 @@ from torched_impala_amd import ops
 
 _TYPES = (torch.float32, torch.bfloat16, torch.float16)
 MAX_HEAD = 128
+MAX_HEADS = ((1 << 32) - 1) // (3 * 512)   # of a batch, as the kernels launch
 
 
 def _check(name, q, k, v, log_decay, done, state, scale, lead):
@@ -51,6 +52,9 @@ def _check(name, q, k, v, log_decay, done, state, scale, lead):
         raise ValueError(f"{name}: head sizes must be 1 to {MAX_HEAD}, "
                          f"not {dk} and {dv}")
     H = q.shape[-2]
+    if q.shape[lead - 1] * H > MAX_HEADS:
+        raise ValueError(f"{name}: batch times heads must be at most "
+                         f"{MAX_HEADS}")
     if log_decay.dtype is not torch.float32:
         raise TypeError(f"{name}: log_decay must be fp32, "
                         f"not {log_decay.dtype}")
@@ -112,7 +116,8 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     """Linear attention over a time-major unroll.
 
     ``q``, ``k`` (T, B, H, dk) and ``v`` (T, B, H, dv) share one type, fp32,
-    bf16 or fp16; head sizes are 1 to 128; T, B or H may be 0. Any strides:
+    bf16 or fp16; head sizes are 1 to 128; T, B or H may be 0, B * H up to
+    2796202 (the threads of a launch). Any strides:
     the three may be parts of one projection, or broadcast over an axis
     (a copy is made only where a head's features are not adjacent).
     ``log_decay`` (H,) fp32 is each head's slope, at most 0; larger values
