@@ -67,7 +67,14 @@ def _close(got, ref, mag, rel, what):
     half = torch.finfo(got.dtype).eps / 2
     tiny = torch.finfo(got.dtype).tiny
     tol = rel * mag * (1 + half) + half * ref.abs() + tiny
-    bad = ~((got.detach().double().cpu() - ref).abs() <= tol)
+    x = got.detach().double().cpu()
+    ok = (x - ref).abs() <= tol
+    # beyond the type's largest value plus half its step a result is infinite,
+    # where the error may reach across that place it may be
+    top = torch.finfo(got.dtype).max * (1 + half / 2)
+    ok &= ref.abs() - tol <= top
+    ok |= (x == ref.sign() * math.inf) & (ref.abs() + tol >= top)
+    bad = ~ok
     assert not bool(bad.any()), (
         what, int(bad.sum()),
         float(((got.detach().double().cpu() - ref).abs() - tol).max()))
@@ -254,6 +261,27 @@ LENGTHS = [1, 2, 15, 16, 17, 21, 33, 48, 63, 64, 65, 101, 128, 129, 200]
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_lengths(T, dtype):
     _check(*_inputs(T, 3, 2, 64, 64, dtype, seed=T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("eq,ek,ev,eo", [(-18, 0, 0, 0), (0, -18, 0, 0),
+                                         (0, 0, -18, 0), (0, 0, 0, -18),
+                                         (-18, -18, -18, -18),
+                                         (12, 12, 12, 12), (12, -18, 12, -18),
+                                         (-18, 12, -18, 12)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_fp16_range(eq, ek, ev, eo, D):
+    """Operands among fp16's subnormals and its largest values: products and
+    states are far beyond fp16's range on both sides, and exact operands
+    stay exact. The scale brings the output back into fp16."""
+    q, k, v, g, d, s, do, df = _inputs(150, 2, 2, D, D, torch.float32, 0.02,
+                                       seed=D + eq + 2 * ek + 3 * ev + 5 * eo)
+    q, k, v, do = (((t * 2.0 ** e).clamp(-60000, 60000)).half()
+                   for t, e in ((q, eq), (k, ek), (v, ev), (do, eo)))
+    s, df = s * 2.0 ** (ek + ev), df * 2.0 ** (eq + eo)
+    # the largest of the four results' exponents at 2^0
+    top = max(eq + ek + ev, eo + ev + ek, eo + ev + eq, eo + ek + eq)
+    _check(q, k, v, g, d, s, do, df, scale=2.0 ** (-5 - top))
 
 
 @pytest.mark.gpu

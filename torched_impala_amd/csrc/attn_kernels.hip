@@ -31,8 +31,11 @@
 // to become an operand again is split into bf16 parts, so that the rounding
 // of operands does not add to that of the result: P and S into two (2^-17,
 // against 2^-9 of the bf16 result), the weighted c of the state update into
-// three (2^-25), because the state is carried on in fp32. fp32 and fp16 run
-// on v_mfma_f32_16x16x4_f32: the range of fp16 does not hold a state.
+// three (2^-25), because the state is carried on in fp32. fp16 runs on
+// v_mfma_f32_16x16x32_f16 at the same rate, except for P c: P does not fit the
+// range of fp16, so both are split into two bf16 parts, c exactly. S and the
+// weighted c are split into two fp16 parts (2^-23) after scaling each column
+// by a power of two (below). fp32 runs on v_mfma_f32_16x16x4_f32.
 //
 // Long sequences of few heads are cut into segments: a first pass leaves
 // every segment's own state, a scan over segments turns them into entry
@@ -61,7 +64,6 @@ namespace attn {
 
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
-typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x4 __attribute__((ext_vector_type(4)));
 typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -95,22 +97,22 @@ struct Decay {
 // operands of a 16 x 16 product over 32 values of k. Lane l = 16 g + m holds
 // row (or column) m; its values are k = 4 g + r and 16 + 4 g + r, r = 0..3:
 // two blocks of a product's result, as they come.
+//
+// L: type in LDS, P: type of the parts of P there. PAD: of a row in LDS, so
+// that rows are 4 banks apart. NP: parts of P and of S as operands, NU: of
+// the weighted c. SCALED: S and the weighted c are brought into the range of
+// their parts by a power of two a column.
 // --------------------------------------------------------------------------
-struct EngineBF16 {
-  typedef bf16_t L;              // type in LDS
-  typedef bf16x8 Frag;
-  static constexpr int PAD = 8;  // row padding in LDS: rows 4 banks apart
-  static constexpr int NP = 2;   // parts of P and of S as operands
-  static constexpr int NU = 3;   // parts of the weighted c
-
-  static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 acc) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
-  }
+template <typename F>
+struct Frag16 {   // reads of 16-bit values
+  typedef F L;
+  typedef F Frag __attribute__((ext_vector_type(8)));
+  typedef F Quad __attribute__((ext_vector_type(4)));
   // rows row0 + m, k along the row
   static __device__ Frag rows(const L* p, int ld, int row0, int k0, int l) {
     const L* q = p + (row0 + (l & 15)) * ld + k0 + 4 * (l >> 4);
-    const bf16x4 x = *reinterpret_cast<const bf16x4*>(q);
-    const bf16x4 y = *reinterpret_cast<const bf16x4*>(q + 16);
+    const Quad x = *reinterpret_cast<const Quad*>(q);
+    const Quad y = *reinterpret_cast<const Quad*>(q + 16);
     return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
   }
   // columns col0 + m, k down the rows: the transposing read. In a group of
@@ -127,22 +129,16 @@ struct EngineBF16 {
     return __builtin_bit_cast(
         Frag, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
   }
-  static __device__ void store4(L* p, int part, f32x4 x) {
-    const bf16x4 h = __builtin_convertvector(x, bf16x4);
-    *reinterpret_cast<bf16x4*>(p) = h;
-    *reinterpret_cast<bf16x4*>(p + part) = __builtin_convertvector(
-        x - __builtin_convertvector(h, f32x4), bf16x4);
-  }
-  static __device__ float at(const Frag& f, int e) { return (float)f[e]; }
-  // fp32 values in N bf16 parts each, two at a time as the hardware converts
+  // fp32 values in N parts each, two at a time as the hardware converts
   template <int N>
   static __device__ void split(const float* v, Frag* out) {
+    typedef F Two __attribute__((ext_vector_type(2)));
     #pragma unroll
     for (int e = 0; e < 8; e += 2) {
       f32x2 x = {v[e], v[e + 1]};
       #pragma unroll
       for (int n = 0; n < N; ++n) {
-        const bf16x2 h = __builtin_convertvector(x, bf16x2);
+        const Two h = __builtin_convertvector(x, Two);
         out[n][e] = h[0];
         out[n][e + 1] = h[1];
         if (n + 1 < N) x -= __builtin_convertvector(h, f32x2);
@@ -151,12 +147,88 @@ struct EngineBF16 {
   }
 };
 
+struct EngineBF16 : Frag16<bf16_t> {
+  typedef bf16_t P;
+  typedef Frag PFrag;
+  typedef Frag CFrag;
+  static constexpr int PAD = 8;
+  static constexpr int NP = 2;
+  static constexpr int NU = 3;
+  static constexpr bool SCALED = false;
+
+  static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc, 0, 0, 0);
+  }
+  static __device__ CFrag c_of(const Frag& f) { return f; }
+  static __device__ float at(const Frag& f, int e) { return (float)f[e]; }
+  static __device__ f32x4 mma_pc(const CFrag& c, const PFrag& p, int,
+                                 f32x4 acc) {
+    return mma(c, p, acc);
+  }
+  static __device__ PFrag p_rows(const P* p, int ld, int row0, int k0,
+                                 int l) {
+    return rows(p, ld, row0, k0, l);
+  }
+  static __device__ void p_split(const float* v, PFrag* out) {
+    split<NP>(v, out);
+  }
+  static __device__ void store4(P* p, int part, f32x4 x) {
+    const bf16x4 h = __builtin_convertvector(x, bf16x4);
+    *reinterpret_cast<bf16x4*>(p) = h;
+    *reinterpret_cast<bf16x4*>(p + part) = __builtin_convertvector(
+        x - __builtin_convertvector(h, f32x4), bf16x4);
+  }
+};
+
+struct EngineF16 : Frag16<f16_t> {
+  typedef EngineBF16 B;
+  typedef bf16_t P;
+  typedef B::Frag PFrag;
+  struct CFrag { B::Frag hi, lo; };
+  static constexpr int PAD = 8;
+  static constexpr int NP = 2;
+  static constexpr int NU = 2;
+  static constexpr bool SCALED = true;
+
+  static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 acc) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, acc, 0, 0, 0);
+  }
+  static __device__ CFrag c_of(const Frag& f) {
+    float v[8];
+    #pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)f[e];
+    B::Frag h[2];
+    B::split<2>(v, h);
+    return CFrag{h[0], h[1]};
+  }
+  static __device__ float at(const Frag& f, int e) { return (float)f[e]; }
+  static __device__ f32x4 mma_pc(const CFrag& c, const PFrag& p, int part,
+                                 f32x4 acc) {
+    if (part == 0) acc = B::mma(c.lo, p, acc);
+    return B::mma(c.hi, p, acc);
+  }
+  static __device__ PFrag p_rows(const P* p, int ld, int row0, int k0,
+                                 int l) {
+    return B::rows(p, ld, row0, k0, l);
+  }
+  static __device__ void p_split(const float* v, PFrag* out) {
+    B::split<NP>(v, out);
+  }
+  static __device__ void store4(P* p, int part, f32x4 x) {
+    B::store4(p, part, x);
+  }
+};
+
 struct EngineF32 {
   typedef float L;
+  typedef float P;
   struct Frag { f32x4 x[2]; };
+  typedef Frag PFrag;
+  typedef Frag CFrag;
   static constexpr int PAD = 4;
   static constexpr int NP = 1;
   static constexpr int NU = 1;
+  static constexpr bool SCALED = false;
 
   static __device__ f32x4 mma(const Frag& a, const Frag& b, f32x4 acc) {
     #pragma unroll
@@ -188,16 +260,48 @@ struct EngineF32 {
   static __device__ void store4(L* p, int, f32x4 x) {
     *reinterpret_cast<f32x4*>(p) = x;
   }
+  static __device__ CFrag c_of(const Frag& f) { return f; }
   static __device__ float at(const Frag& f, int e) { return f.x[e >> 2][e & 3]; }
+  static __device__ f32x4 mma_pc(const CFrag& c, const PFrag& p, int,
+                                 f32x4 acc) {
+    return mma(c, p, acc);
+  }
+  static __device__ PFrag p_rows(const P* p, int ld, int row0, int k0,
+                                 int l) {
+    return rows(p, ld, row0, k0, l);
+  }
   template <int N>
   static __device__ void split(const float* v, Frag* out) {
     #pragma unroll
     for (int e = 0; e < 8; ++e) out[0].x[e >> 2][e & 3] = v[e];
   }
+  static __device__ void p_split(const float* v, PFrag* out) {
+    split<1>(v, out);
+  }
 };
 
 template <typename T> struct EngineOf { typedef EngineF32 E; };
 template <> struct EngineOf<bf16_t> { typedef EngineBF16 E; };
+template <> struct EngineOf<f16_t> { typedef EngineF16 E; };
+
+// A power of two that brings a column's largest value to 2^14..2^15, and its
+// reciprocal. Two fp16 parts then hold a value to 2^-23, down to 2^-17 of the
+// column's largest; smaller ones are off by 2^-40 of that largest at most.
+// (fp32 products instead, without any of this: 316 us against 146 forward for
+// T=16384, B=2, 8 heads of 128.) top: the largest magnitude in this lane; a
+// column's four lanes agree on it. Columns below 2^-87 are scaled as if they
+// reached it. Infinities and NaN stay what they are.
+struct Scale {
+  float to, from;
+  __device__ explicit Scale(float top) {
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    int e = (int)(__builtin_bit_cast(unsigned, top) >> 23);
+    e = e > 40 ? e : 40;
+    to = __builtin_bit_cast(float, (unsigned)(268 - e) << 23);
+    from = __builtin_bit_cast(float, (unsigned)(e - 14) << 23);
+  }
+};
 
 // How a workgroup divides its work: NV blocks of 16 value columns a wave, and
 // whether the waves share the blocks of P through LDS or each computes all of
@@ -211,6 +315,12 @@ template <typename T, int D> struct Split {
 };
 template <int D> struct Split<bf16_t, D> {
   static constexpr int NV = D > 64 ? 1 : 2;
+  static constexpr bool SHARE = D > 64;
+};
+// fp16 has more of its own to keep in registers: with two blocks it spills
+// (51 us against 49 with one, the same case; 31 against 28 for heads of 32).
+template <int D> struct Split<f16_t, D> {
+  static constexpr int NV = 1;
   static constexpr bool SHARE = D > 64;
 };
 
@@ -253,8 +363,7 @@ struct Rows {
       }
     }
   }
-  template <typename LT>
-  __device__ void store(LT* s, int ld, int len, int d) {
+  __device__ void store(T* s, int ld, int len, int d) {
     if (len < C || d < D) {
       #pragma unroll
       for (int n = 0; n < N; ++n) {
@@ -267,22 +376,10 @@ struct Rows {
         }
       }
     }
-    LT* p = s + row * ld + col;
+    T* p = s + row * ld + col;
     #pragma unroll
-    for (int n = 0; n < N; ++n) {
-      LT* q = p + n * STEP * ld;
-      if constexpr (sizeof(LT) == sizeof(T)) {
-        *reinterpret_cast<u32x4*>(q) = r[n].q;
-      } else {   // fp16 in fp32
-        #pragma unroll
-        for (int e = 0; e < V; e += 4) {
-          f32x4 f;
-          #pragma unroll
-          for (int k = 0; k < 4; ++k) f[k] = (float)r[n].v[e + k];
-          *reinterpret_cast<f32x4*>(q + e) = f;
-        }
-      }
-    }
+    for (int n = 0; n < N; ++n)
+      *reinterpret_cast<u32x4*>(p + n * STEP * ld) = r[n].q;
   }
 };
 
@@ -304,6 +401,7 @@ attn_chunks(AttnArgs args) {
   typedef typename EngineOf<T>::E E;
   typedef typename E::L L;
   typedef typename E::Frag Frag;
+  typedef typename E::PFrag PFrag;
   constexpr int THREADS = threads_of<T, D>();
   constexpr int NW = THREADS / 64;   // waves
   constexpr int NV = Split<T, D>::NV;   // 16-column blocks of a wave's values
@@ -317,7 +415,7 @@ attn_chunks(AttnArgs args) {
   __shared__ __align__(16) L sa[STATE_ONLY ? 1 : C * LD];
   __shared__ __align__(16) L sb[C * LD];
   __shared__ __align__(16) L sc[C * LD];
-  __shared__ __align__(16) L sp[SHARE ? E::NP * PART : 8];
+  __shared__ __align__(16) typename E::P sp[SHARE ? E::NP * PART : 8];
   __shared__ float pw[C + 1];
   __shared__ __align__(16) float w_out[C];
   __shared__ float w_in[C];
@@ -451,7 +549,7 @@ attn_chunks(AttnArgs args) {
   for (int i = tid; i <= C; i += THREADS) pw[i] = decay.pow((float)i);
   if constexpr (SHARE) {   // blocks of P that the mask leaves out stay zero
     u32x4* z = reinterpret_cast<u32x4*>(sp);
-    constexpr int NZ = E::NP * PART * (int)sizeof(L) / 16;
+    constexpr int NZ = E::NP * PART * (int)sizeof(typename E::P) / 16;
     for (int i = tid; i < NZ; i += THREADS) z[i] = u32x4{0, 0, 0, 0};
   }
   bool seen_done = false;
@@ -564,6 +662,24 @@ attn_chunks(AttnArgs args) {
           for (int v = 0; v < NV; ++v) O[it][v] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
         if (any_state) {
+          float to[NV], back[NV][4];   // of S: a column is a row of O
+          if constexpr (E::SCALED) {
+            #pragma unroll
+            for (int v = 0; v < NV; ++v) {
+              float top = 0.f;
+              #pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                #pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  top = fmaxf(top, fabsf(S[t][v][r]));
+              }
+              const Scale scale(top);
+              to[v] = scale.to;
+              #pragma unroll
+              for (int r = 0; r < 4; ++r)
+                back[v][r] = __shfl(scale.from, 4 * g + r, 64);
+            }
+          }
           #pragma unroll
           for (int s = 0; s < NS; ++s) {
             Frag sf[NV][E::NP];
@@ -574,6 +690,10 @@ attn_chunks(AttnArgs args) {
               for (int r = 0; r < 4; ++r) {
                 x[r] = S[2 * s][v][r];
                 x[4 + r] = S[2 * s + 1][v][r];
+                if constexpr (E::SCALED) {
+                  x[r] *= to[v];
+                  x[4 + r] *= to[v];
+                }
               }
               E::template split<E::NP>(x, sf[v]);
             }
@@ -594,7 +714,10 @@ attn_chunks(AttnArgs args) {
             #pragma unroll
             for (int v = 0; v < NV; ++v) {
               #pragma unroll
-              for (int r = 0; r < 4; ++r) O[it][v][r] *= w;
+              for (int r = 0; r < 4; ++r) {
+                if constexpr (E::SCALED) O[it][v][r] *= back[v][r];
+                O[it][v][r] *= w;
+              }
             }
           }
         }
@@ -610,6 +733,12 @@ attn_chunks(AttnArgs args) {
     if constexpr (SHARE) __syncthreads();   // P is whole
     if (!idle) {
       if constexpr (!STATE_ONLY) {
+        typename E::CFrag cc[2][NV];
+        #pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          #pragma unroll
+          for (int v = 0; v < NV; ++v) cc[s][v] = E::c_of(cf[s][v]);
+        }
         // row blocks 0 and 1 meet the first 32 rows of j, 2 and 3 all
         #pragma unroll
         for (int it = 0; it < 4; ++it) {
@@ -618,11 +747,11 @@ attn_chunks(AttnArgs args) {
             for (int s = 0; s <= it >> 1; ++s) {
               #pragma unroll
               for (int p = 0; p < E::NP; ++p) {
-                const Frag pf =
-                    E::rows(sp + p * PART, LDP, 16 * it, 32 * s, l);
+                const PFrag pf =
+                    E::p_rows(sp + p * PART, LDP, 16 * it, 32 * s, l);
                 #pragma unroll
                 for (int v = 0; v < NV; ++v)
-                  O[it][v] = E::mma(cf[s][v], pf, O[it][v]);
+                  O[it][v] = E::mma_pc(cc[s][v], pf, p, O[it][v]);
               }
             }
           } else {
@@ -662,13 +791,13 @@ attn_chunks(AttnArgs args) {
                 x[r] = acc[2 * s][r];
                 x[4 + r] = acc[2 * s + 1][r];
               }
-              Frag pf[E::NP];
-              E::template split<E::NP>(x, pf);
+              PFrag pf[E::NP];
+              E::p_split(x, pf);
               #pragma unroll
               for (int p = 0; p < E::NP; ++p) {
                 #pragma unroll
                 for (int v = 0; v < NV; ++v)
-                  O[it][v] = E::mma(cf[s][v], pf[p], O[it][v]);
+                  O[it][v] = E::mma_pc(cc[s][v], pf[p], p, O[it][v]);
               }
             }
           }
@@ -728,7 +857,23 @@ attn_chunks(AttnArgs args) {
           #pragma unroll
           for (int v = 0; v < NV; ++v) {
             #pragma unroll
-            for (int r = 0; r < 4; ++r) U[t][v][r] = S[t][v][r] * keep;
+            for (int r = 0; r < 4; ++r)
+              U[t][v][r] = E::SCALED ? 0.f : S[t][v][r] * keep;
+          }
+        }
+        float to[NV], from[NV];   // of the weighted c
+        if constexpr (E::SCALED) {
+          #pragma unroll
+          for (int v = 0; v < NV; ++v) {
+            float top = 0.f;
+            #pragma unroll
+            for (int e = 0; e < 16; ++e)
+              top = fmaxf(top, fabsf(E::at(cf[e >> 3][v], e & 7) *
+                                     w_out[32 * (e >> 3) + 16 * (e >> 2 & 1) +
+                                           4 * g + (e & 3)]));
+            const Scale scale(top);
+            to[v] = scale.to;
+            from[v] = scale.from;
           }
         }
         #pragma unroll
@@ -742,8 +887,10 @@ attn_chunks(AttnArgs args) {
           for (int v = 0; v < NV; ++v) {
             float x[8];
             #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              x[e] = E::at(cf[s][v], e) * (e < 4 ? w0[e & 3] : w1[e & 3]);
+            for (int e = 0; e < 8; ++e) {
+              const float w = e < 4 ? w0[e & 3] : w1[e & 3];
+              x[e] = E::at(cf[s][v], e) * (E::SCALED ? w * to[v] : w);
+            }
             E::template split<E::NU>(x, cw[v]);
           }
           #pragma unroll
@@ -754,6 +901,17 @@ attn_chunks(AttnArgs args) {
               #pragma unroll
               for (int v = 0; v < NV; ++v)
                 U[t][v] = E::mma(bf, cw[v][p], U[t][v]);
+            }
+          }
+        }
+        if constexpr (E::SCALED) {
+          #pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            #pragma unroll
+            for (int v = 0; v < NV; ++v) {
+              #pragma unroll
+              for (int r = 0; r < 4; ++r)
+                U[t][v][r] = fmaf(U[t][v][r], from[v], S[t][v][r] * keep);
             }
           }
         }
