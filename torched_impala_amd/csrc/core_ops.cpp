@@ -654,42 +654,65 @@ int scale_exp(long n) {
   return e < 13 ? e : 13;
 }
 
+int k_step(int tile) { return tile == 64 ? 64 : 32; }
+
+long k_steps(const ns::Mat& m, int mode, int tile) {
+  return (mode == 0 ? m.np : m.mp) / k_step(tile);
+}
+
+int tiles_of(const ns::Mat& m, int mode, int tile) {
+  const int tm = m.mp / tile, tn = m.np / tile;
+  return mode == 2 ? tm * tn : tm * (tm + 1) / 2;
+}
+
+// Steps of k that a block takes; what is longer is split over blocks, whose
+// parts a second launch adds. Least of an estimate in us, from measured
+// products: a step takes a block alone on a CU 1.3 (tiles of 128) or 0.65, two
+// on a CU 1.5 or 0.9, and 1.9 or 1.1 where more than the 512 that run at once
+// keep all of the card busy; adding takes 6 and the parts' bytes at 2 MB a
+// us. Six products of 1024^3: unsplit 47, split in two
+// 35 + 16. 10 tiles of 64 over k = 1568: unsplit 21, in four 9 + 7, in seven
+// 7 + 6. 2048 x 2048 and 2048 x 8192: k in steps of 4096 193 + 14, of 1024
+// 202 + 31.
+long block_steps(const ns::Args& a, int mode, int tile) {
+  const double alone = tile == 64 ? 0.65 : 1.3;
+  const double both = tile == 64 ? 0.9 : 1.5, full = tile == 64 ? 1.1 : 1.9;
+  long longest = 0;
+  for (int i = 0; i < a.count; ++i)
+    longest = std::max(longest, k_steps(a.mat[i], mode, tile));
+  long best = longest;
+  double least = 1e30;
+  for (long n = 1; n <= 64; ++n) {
+    const long per = (longest + n - 1) / n;
+    if (n > 1 && per * k_step(tile) < 256) break;
+    long blocks = 0, parts = 0;
+    for (int i = 0; i < a.count; ++i) {
+      const long splits = (k_steps(a.mat[i], mode, tile) + per - 1) / per;
+      const long mine = splits * tiles_of(a.mat[i], mode, tile);
+      blocks += mine;
+      if (splits > 1) parts += mine;
+    }
+    const double t = per * (blocks <= 256   ? alone
+                            : blocks <= 512 ? both
+                                            : (blocks + 511) / 512 * full) +
+                     (parts ? 6.0 + parts * 4.0 * tile * tile / 2e6 : 0.0);
+    if (t < least) {
+      least = t;
+      best = per;
+    }
+  }
+  return best;
+}
+
 // tiles of one product of all matrices, and the blocks that share a tile's k;
 // returns the floats that the parts of split tiles need
-long plan_product(ns::Args& a, int mode, int tile) {
-  const int ks = tile == 64 ? 64 : 32;
-  // blocks that run at once: two a CU fit its LDS
-  const long slots = 512;
-  long total = 0, work = 0, longest = 0;
-  for (int i = 0; i < a.count; ++i) {
-    ns::Mat& m = a.mat[i];
-    const int tm = m.mp / tile, tn = m.np / tile;
-    m.tiles = mode == 2 ? tm * tn : tm * (tm + 1) / 2;
-    const long steps = (mode == 0 ? m.np : m.mp) / ks;
-    total += m.tiles;
-    work += m.tiles * steps;
-    longest = std::max(longest, steps);
-  }
-  // Steps of k for a block so that all blocks run at once, 512 values at
-  // least: below that, adding the parts costs more than it saves. Nothing is
-  // split where the blocks fill the card anyway or the gain is small.
-  long per = std::max((work + slots - 1) / slots, 512L / ks);
-  auto blocks_at = [&](long steps_a_block) {
-    long n = 0;
-    for (int i = 0; i < a.count; ++i)
-      n += a.mat[i].tiles *
-           (((mode == 0 ? a.mat[i].np : a.mat[i].mp) / ks + steps_a_block -
-             1) / steps_a_block);
-    return n;
-  };
-  while (per < longest && blocks_at(per) > slots) ++per;
-  if (total >= slots || longest * 2 <= per * 3) per = longest;
+long plan_product(ns::Args& a, int mode, int tile, long per) {
   long part = 0;
   int blocks = 0, sums = 0;
   for (int i = 0; i < a.count; ++i) {
     ns::Mat& m = a.mat[i];
-    const long steps = (mode == 0 ? m.np : m.mp) / ks;
-    m.splits = (int)((steps + per - 1) / per);
+    m.tiles = tiles_of(m, mode, tile);
+    m.splits = (int)((k_steps(m, mode, tile) + per - 1) / per);
     a.first[i] = blocks;
     a.first_sum[i] = sums;
     a.part_off[i] = part;
@@ -774,9 +797,11 @@ void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
       norm_blocks += m.norm_blocks;
     }
     a.first_norm[a.count] = norm_blocks;
-    long partial = 0;
-    for (int mode = 0; mode < 3; ++mode)
-      partial = std::max(partial, plan_product(a, mode, tile));
+    long partial = 0, per[3];
+    for (int mode = 0; mode < 3; ++mode) {
+      per[mode] = block_steps(a, mode, tile);
+      partial = std::max(partial, plan_product(a, mode, tile, per[mode]));
+    }
     auto work = torch::empty({parts}, like.options().dtype(torch::kFloat16));
     auto split = torch::empty({partial},
                               like.options().dtype(torch::kFloat32));
@@ -793,7 +818,7 @@ void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
       a.round = (int)k;
       a.last = k + 1 == steps;
       for (int mode = 0; mode < 3; ++mode) {
-        plan_product(a, mode, tile);
+        plan_product(a, mode, tile, per[mode]);
         launch_ns_product(mode, tile, &a, stream);
       }
     }

@@ -20,10 +20,12 @@
 // eps), times a each round, up to 1.25), so its entries are of the order of
 // beta_k / sqrt(n), and those of A of beta_k^2 / sqrt(m).
 //
-// Measured, a round of 2048 x 2048 and 2048 x 8192: 206 us for A, 112 for B,
-// 340 for X (0.76 PFLOP/s of fp16 products, where the library's large bf16
+// Measured, a round of 2048 x 2048 and 2048 x 8192: 193 us for A, 110 for B,
+// 299 for X (0.86 PFLOP/s of fp16 products, where the library's large bf16
 // product reaches 1.05), 14 for adding parts. A round of the shallow net's
-// matrices (6, up to 1024 x 263 and 256 x 1568) takes 38 us, about 10 a launch.
+// matrices (6, up to 1024 x 263 and 256 x 1568) takes 35 us, about 9 a launch
+// with an empty one at 2: arguments, first operands and last results come and
+// go once a launch.
 //
 // A and B are symmetric: only tiles on and under the diagonal are computed,
 // and written twice. X is kept in both orientations, so that every product
@@ -288,10 +290,11 @@ __device__ inline void finish(const Args& args, int mi, int ti, int tj,
 // One product, C = P Q^T over k, P and Q in two parts with k contiguous.
 // MODE 0: A = X X^T. MODE 1: B = a I + b A + c A A. MODE 2: X = B X.
 // TILE x TILE of C a block, four waves of half that each way; k in steps of
-// KS through two LDS buffers, the next step's rows on their way in registers.
+// KS through two LDS buffers, the rows of the next DEPTH steps on their way in
+// registers (one step: 340 us for X above; three: as two).
 // Few tiles of long k are split over blocks; a second launch adds their parts
 // (letting the last block of a tile add them costs a write-back of the L2 a
-// block: 175 us against 35 + 18 for six matrices of 1024).
+// block: 175 us against 35 + 16 for six matrices of 1024).
 // --------------------------------------------------------------------------
 template <int MODE, int TILE>
 __global__ void __launch_bounds__(256) ns_product(Args args) {
@@ -327,28 +330,32 @@ __global__ void __launch_bounds__(256) ns_product(Args args) {
   const int k_lo = split * per;
   const int k_hi = k_lo + per < steps ? k_lo + per : steps;
 
-  u32x4 r0[PIECES], r1[PIECES], r2[PIECES], r3[PIECES];
-  auto fetch = [&](int step) __attribute__((always_inline)) {
+  constexpr int DEPTH = 2;
+  u32x4 r0[DEPTH][PIECES], r1[DEPTH][PIECES], r2[DEPTH][PIECES],
+      r3[DEPTH][PIECES];
+  // behind the last step that one is read again, and not used
+  auto fetch = [&](int d, int step) __attribute__((always_inline)) {
+    step = step < k_hi ? step : k_hi - 1;
     #pragma unroll
     for (int n = 0; n < PIECES; ++n) {
       const int idx = n * 256 + tid;
       const long off =
           (long)(idx / PER_ROW) * K + step * KS + (idx % PER_ROW) * 8;
-      r0[n] = *reinterpret_cast<const u32x4*>(P + off);
-      r1[n] = *reinterpret_cast<const u32x4*>(P + plane_p + off);
-      r2[n] = *reinterpret_cast<const u32x4*>(Q + off);
-      r3[n] = *reinterpret_cast<const u32x4*>(Q + plane_q + off);
+      r0[d][n] = *reinterpret_cast<const u32x4*>(P + off);
+      r1[d][n] = *reinterpret_cast<const u32x4*>(P + plane_p + off);
+      r2[d][n] = *reinterpret_cast<const u32x4*>(Q + off);
+      r3[d][n] = *reinterpret_cast<const u32x4*>(Q + plane_q + off);
     }
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
+  auto put = [&](int d, int buf) __attribute__((always_inline)) {
     #pragma unroll
     for (int n = 0; n < PIECES; ++n) {
       const int idx = n * 256 + tid;
       const int at = (idx / PER_ROW) * LD + (idx % PER_ROW) * 8;
-      *reinterpret_cast<u32x4*>(&lds[buf][0][at]) = r0[n];
-      *reinterpret_cast<u32x4*>(&lds[buf][1][at]) = r1[n];
-      *reinterpret_cast<u32x4*>(&lds[buf][2][at]) = r2[n];
-      *reinterpret_cast<u32x4*>(&lds[buf][3][at]) = r3[n];
+      *reinterpret_cast<u32x4*>(&lds[buf][0][at]) = r0[d][n];
+      *reinterpret_cast<u32x4*>(&lds[buf][1][at]) = r1[d][n];
+      *reinterpret_cast<u32x4*>(&lds[buf][2][at]) = r2[d][n];
+      *reinterpret_cast<u32x4*>(&lds[buf][3][at]) = r3[d][n];
     }
   };
 
@@ -358,40 +365,43 @@ __global__ void __launch_bounds__(256) ns_product(Args args) {
     #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  if (k_lo < k_hi) {
-    fetch(k_lo);
-    put(0);
-  }
-  for (int k = k_lo; k < k_hi; ++k) {
-    const int buf = (k - k_lo) & 1;
-    __syncthreads();
-    if (k + 1 < k_hi) fetch(k + 1);
+  #pragma unroll
+  for (int d = 0; d < DEPTH; ++d) fetch(d, k_lo + d);
+  int buf = 0;
+  for (int k0 = k_lo; k0 < k_hi; k0 += DEPTH) {
     #pragma unroll
-    for (int s = 0; s < KS / 32; ++s) {
-      halfx8 ph[NF], pl[NF], qh[NF], ql[NF];
+    for (int d = 0; d < DEPTH; ++d) {
+      if (k0 + d >= k_hi) break;
+      put(d, buf);
+      fetch(d, k0 + d + DEPTH);
+      __syncthreads();
       #pragma unroll
-      for (int i = 0; i < NF; ++i) {
-        const int pa = (wi + 16 * i + m) * LD + 32 * s + 8 * g;
-        const int qa = (wj + 16 * i + m) * LD + 32 * s + 8 * g;
-        ph[i] = *reinterpret_cast<const halfx8*>(&lds[buf][0][pa]);
-        pl[i] = *reinterpret_cast<const halfx8*>(&lds[buf][1][pa]);
-        qh[i] = *reinterpret_cast<const halfx8*>(&lds[buf][2][qa]);
-        ql[i] = *reinterpret_cast<const halfx8*>(&lds[buf][3][qa]);
-      }
-      #pragma unroll
-      for (int i = 0; i < NF; ++i) {
+      for (int s = 0; s < KS / 32; ++s) {
+        halfx8 ph[NF], pl[NF], qh[NF], ql[NF];
         #pragma unroll
-        for (int j = 0; j < NF; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              ph[i], qh[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              ph[i], ql[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-              pl[i], qh[j], acc[i][j], 0, 0, 0);
+        for (int i = 0; i < NF; ++i) {
+          const int pa = (wi + 16 * i + m) * LD + 32 * s + 8 * g;
+          const int qa = (wj + 16 * i + m) * LD + 32 * s + 8 * g;
+          ph[i] = *reinterpret_cast<const halfx8*>(&lds[buf][0][pa]);
+          pl[i] = *reinterpret_cast<const halfx8*>(&lds[buf][1][pa]);
+          qh[i] = *reinterpret_cast<const halfx8*>(&lds[buf][2][qa]);
+          ql[i] = *reinterpret_cast<const halfx8*>(&lds[buf][3][qa]);
+        }
+        #pragma unroll
+        for (int i = 0; i < NF; ++i) {
+          #pragma unroll
+          for (int j = 0; j < NF; ++j) {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                ph[i], qh[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                ph[i], ql[j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                pl[i], qh[j], acc[i][j], 0, 0, 0);
+          }
         }
       }
+      buf ^= 1;
     }
-    if (k + 1 < k_hi) put(buf ^ 1);
   }
 
   if (M.splits > 1) {   // ns_sum adds the parts
@@ -420,16 +430,21 @@ __global__ void __launch_bounds__(256) ns_sum(Args args) {
   place<MODE, TILE>(M, tile, &ti, &tj);
   const float* base = args.partial + args.part_off[mi] +
                       (long)tile * M.splits * TILE * TILE;
+  // all places of a part at once: one by one each waits for memory
   f32x4 acc[NF][NF];
   #pragma unroll
   for (int i = 0; i < NF; ++i) {
     #pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const float* p = base + ((i * NF + j) * 256 + threadIdx.x) * 4;
-      f32x4 sum = *reinterpret_cast<const f32x4*>(p);
-      for (int s = 1; s < M.splits; ++s)
-        sum += *reinterpret_cast<const f32x4*>(p + (long)s * TILE * TILE);
-      acc[i][j] = sum;
+    for (int j = 0; j < NF; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  #pragma unroll 2
+  for (int s = 0; s < M.splits; ++s) {
+    const float* p = base + (long)s * TILE * TILE + threadIdx.x * 4;
+    #pragma unroll
+    for (int i = 0; i < NF; ++i) {
+      #pragma unroll
+      for (int j = 0; j < NF; ++j)
+        acc[i][j] += *reinterpret_cast<const f32x4*>(p + (i * NF + j) * 1024);
     }
   }
   finish<MODE, TILE>(args, mi, ti, tj, acc);
