@@ -291,13 +291,15 @@ __device__ inline void finish(const Args& args, int mi, int ti, int tj,
 // MODE 0: A = X X^T. MODE 1: B = a I + b A + c A A. MODE 2: X = B X.
 // TILE x TILE of C a block, four waves of half that each way; k in steps of
 // KS through two LDS buffers, the rows of the next DEPTH steps on their way in
-// registers (one step: 340 us for X above; three: as two).
+// registers (one step: 340 us for X above; three: as two). Two blocks a CU
+// have to fit: left to itself the compiler takes registers for one (3775 us
+// against 3063 for five rounds of the matrices above).
 // Few tiles of long k are split over blocks; a second launch adds their parts
 // (letting the last block of a tile add them costs a write-back of the L2 a
 // block: 175 us against 35 + 16 for six matrices of 1024).
 // --------------------------------------------------------------------------
 template <int MODE, int TILE>
-__global__ void __launch_bounds__(256) ns_product(Args args) {
+__global__ void __launch_bounds__(256, 2) ns_product(Args args) {
   constexpr int KS = TILE == 64 ? 64 : 32;
   constexpr int LD = KS + 8;              // rows 4 banks apart
   constexpr int W = TILE / 2, NF = W / 16;
@@ -388,15 +390,14 @@ __global__ void __launch_bounds__(256) ns_product(Args args) {
           ql[i] = *reinterpret_cast<const halfx8*>(&lds[buf][3][qa]);
         }
         #pragma unroll
-        for (int i = 0; i < NF; ++i) {
+        for (int part = 0; part < 3; ++part) {
           #pragma unroll
-          for (int j = 0; j < NF; ++j) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                ph[i], qh[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                ph[i], ql[j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                pl[i], qh[j], acc[i][j], 0, 0, 0);
+          for (int i = 0; i < NF; ++i) {
+            #pragma unroll
+            for (int j = 0; j < NF; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                  part < 2 ? ph[i] : pl[i], part == 1 ? ql[j] : qh[j],
+                  acc[i][j], 0, 0, 0);
           }
         }
       }
