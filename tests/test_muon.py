@@ -8,6 +8,8 @@ norm times the number of rounds' products at these sizes). The update enters
 the weights times the rate.
 """
 import math
+import os
+import queue
 
 import pytest
 import torch
@@ -151,6 +153,68 @@ def test_state_dict_roundtrip():
     with pytest.raises(ValueError):
         ob.load_state_dict(FlatRMSprop(MLPPolicy((4,), 2).parameters())
                            .state_dict())
+
+
+def _train_rank(rank, world, port, q):
+    """Three steps of a linear-attention policy on this rank's half of the
+    batch (world 2) or on all of it (world 1)."""
+    from torched_impala_amd.parallel import FlatGradReducer
+    if world > 1:
+        os.environ["MASTER_ADDR"] = "127.0.0.1"
+        os.environ["MASTER_PORT"] = str(port)
+        torch.distributed.init_process_group("gloo", rank=rank,
+                                             world_size=world)
+    try:
+        torch.manual_seed(0)
+        net = MLPPolicy((4,), 2, use_linear_attention=True)
+        opt = FlatMuon(net.parameters(), muon_matrices(net), lr=0.01,
+                       max_grad_norm=1e6, world_size=world, muon_lr=0.02)
+        red = FlatGradReducer(net, opt, bucket_bytes=1 << 14)
+        for it in range(3):
+            torch.manual_seed(50 + it)
+            x, done = torch.randn(5, 4, 4), torch.rand(5, 4) < 0.2
+            mine = slice(2 * rank, 2 * rank + 2) if world > 1 else slice(0, 4)
+            n = mine.stop - mine.start
+            inputs = dict(frame=x[:, mine], reward=torch.zeros(5, n),
+                          done=done[:, mine],
+                          last_action=torch.zeros(5, n, dtype=torch.long))
+            opt.zero_grad()
+            red.prepare()
+            out, _ = net(inputs, net.initial_state(n))
+            ((out["policy_logits"].pow(2).sum()
+              + out["baseline"].pow(2).sum()) * (world / 2)).backward()
+            red.finalize()
+            opt.step()
+        q.put((rank, opt.flat_param.detach().numpy().copy()))
+    finally:
+        if world > 1:
+            torch.distributed.destroy_process_group()
+
+
+@pytest.mark.timeout(180)
+def test_two_ranks_as_one():
+    """Data parallel over two ranks: the ranks end with the same bits, and
+    with what one process gets from the whole batch (its loss halved, as the
+    ranks' mean is). The sums differ in order only: 20 rows through 8 layers
+    are 2^-19 of a gradient's norm at most. A step's products enlarge that 485
+    times, at a rate of 0.02; RMSProp moves by at most the error over eps =
+    0.01 at a rate of 0.01, with norms up to 10. Over three steps together
+    under 1.2e-4; a rank left out would move weights by 0.02."""
+    ctx = torch.multiprocessing.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_train_rank, args=(r, 2, 29643, q))
+             for r in range(2)]
+    for p in procs:
+        p.start()
+    got = dict(q.get(timeout=120) for _ in range(2))
+    for p in procs:
+        p.join(timeout=30)
+    assert (got[0] == got[1]).all()
+    alone = queue.Queue()
+    _train_rank(0, 1, 0, alone)
+    torch.testing.assert_close(
+        torch.from_numpy(got[0]), torch.from_numpy(alone.get()[1]),
+        rtol=0, atol=1.2e-4)
 
 
 @pytest.mark.gpu
