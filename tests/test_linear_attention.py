@@ -357,6 +357,67 @@ def test_extreme_decays(g, T):
     _check(*a)
 
 
+HALF = torch.float16
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,B,H,dk,dv", [(512, 2, 2, 24, 16),
+                                         (1111, 40, 2, 24, 16),
+                                         (900, 1, 2, 128, 96),
+                                         (700, 1, 3, 64, 64)])
+def test_fp16_cut_into_segments(T, B, H, dk, dv):
+    _check(*_inputs(T, B, H, dk, dv, HALF, 0.002, seed=T))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [[0], [63], [64], [149], [62, 63, 64],
+                                  list(range(150)), [127, 128]])
+def test_fp16_done_places(rows):
+    _check(*_with_done(rows, dtype=HALF))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g", [0.0, -1e-7, -1.0, -30.0, -200.0,
+                               float("-inf")])
+@pytest.mark.parametrize("T", [20, 200, 600])
+@pytest.mark.parametrize("D", [16, 128])
+def test_fp16_extreme_decays(g, T, D):
+    a = _inputs(T, 1, 2, D, D, HALF)
+    a[3] = torch.tensor([g, -0.1], device="cuda")
+    _check(*a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [48, 128])
+def test_padded_rows(dtype, D):
+    """Rows of zeros at the end, or everywhere: what is left of the rows in
+    front has decayed far below one and is still exact."""
+    for rows in (30, 90, 150):
+        a = _inputs(150, 2, 2, D, D, dtype, 0, seed=rows)
+        for t in (a[0], a[1], a[2], a[6]):
+            t[150 - rows:] = 0
+        a[3] = torch.tensor([-1.0, -0.2], device="cuda")
+        _check(*a)
+        a[5] = a[7] = None
+        _check(*a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("e,scale", [(100, 2.0 ** -104), (-100, 1.0),
+                                     (-140, 1.0), (40, 2.0 ** -44)])
+@pytest.mark.parametrize("D", [32, 128])
+def test_states_beyond_the_operands_range(dtype, e, scale, D):
+    """States and their gradients are fp32: their values may be far outside
+    fp16's range."""
+    q, k, v, g, d, s, do, df = _inputs(140, 2, 2, D, D, dtype, 0.02, seed=D)
+    df = df * 2.0 ** min(e, 0)
+    _check(q, k, v, g, d, s * 2.0 ** e, do, df, scale=scale)
+    z = torch.zeros_like
+    _check(q, z(k), v, g, d, s * 2.0 ** e, do, df, scale=scale)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("scale", [0.0, 1.0, -0.3])
 def test_scale(scale):
@@ -452,8 +513,9 @@ def test_non_finite_stays_where_it_belongs(dtype, T, value):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("T", [60, 600])
-def test_non_finite_gradients_stay(T):
-    q, k, v, g, _, s, do, df = _inputs(T, 2, 2, 32, 32, torch.bfloat16)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, HALF])
+def test_non_finite_gradients_stay(T, dtype):
+    q, k, v, g, _, s, do, df = _inputs(T, 2, 2, 32, 32, dtype)
     d = torch.zeros(T, 2, dtype=torch.bool, device="cuda")
     cut = T // 2
     d[cut] = True
