@@ -502,6 +502,14 @@ void with_plan_nv(const Plan& p, F&& f) {
   }
 }
 
+// a block a row takes rows that a wave, and 512 threads those that 256 cannot
+// hold: what a thread then holds is more than a quarter, or half, of the most
+template <int VEC, int NV>
+constexpr bool block_fits(int block) {
+  constexpr int most = VEC == 1 ? MAXPT1 : MAXPT / VEC;
+  return block == 256 ? 4 * NV > most : 2 * NV > most;
+}
+
 template <typename T, typename W, int VEC, int NV>
 void run_fwd(const Plan& p, const void* x, long xs, const void* w,
              const void* b, void* y, float* mean, float* rstd, long rows,
@@ -512,8 +520,12 @@ void run_fwd(const Plan& p, const void* x, long xs, const void* w,
                      dim3(THREADS), 0, s, (const T*)x, xs, (const W*)w,     \
                      (const W*)b, (T*)y, mean, rstd, rows, cols, eps, p.g)
   if (p.block == 0) IMPALA_LN_FWD(0, 256);
-  else if (p.block == 256) IMPALA_LN_FWD(256, 256);
-  else IMPALA_LN_FWD(512, 512);
+  if constexpr (block_fits<VEC, NV>(256)) {
+    if (p.block == 256) IMPALA_LN_FWD(256, 256);
+  }
+  if constexpr (block_fits<VEC, NV>(512)) {
+    if (p.block == 512) IMPALA_LN_FWD(512, 512);
+  }
 #undef IMPALA_LN_FWD
 }
 
@@ -530,8 +542,12 @@ void run_bwd(const Plan& p, const void* dy, const void* x, long xs,
                      dim3(THREADS), lds, s, (const T*)dy, (const T*)x, xs,  \
                      (const W*)w, mean, rstd, (T*)dx, part, rows, cols, p.g)
   if (p.block == 0) IMPALA_LN_BWD(0, 256);
-  else if (p.block == 256) IMPALA_LN_BWD(256, 256);
-  else IMPALA_LN_BWD(512, 512);
+  if constexpr (block_fits<VEC, NV>(256)) {
+    if (p.block == 256) IMPALA_LN_BWD(256, 256);
+  }
+  if constexpr (block_fits<VEC, NV>(512)) {
+    if (p.block == 512) IMPALA_LN_BWD(512, 512);
+  }
 #undef IMPALA_LN_BWD
 }
 
