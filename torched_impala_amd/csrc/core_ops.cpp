@@ -332,13 +332,17 @@ bool can_vec(const Tensor& t, const AttnOperand& o) {
 
 // Segments that a sequence is cut into. Workgroups that run at once: what a
 // CU holds of the kernel's tiles (one of those for heads above 64, whose LDS
-// or registers fill it, two in fp32, four in 16 bits), times 256. Heads that
-// fill those by themselves are not cut. Else n segments take about
-// chunks / n * 9 us for their two passes and n states of all heads, moved five
-// times at 4 MB a us; the sum is least at the root below.
+// or registers fill it, else two, or four of the small ones of bf16 and of fp16
+// up to heads of 32; fp16, T=4096, B=4, 8 heads of 64: 45 us with two, 51 with
+// four; T=2048, B=12, 4 heads of 32: 30 and 26), times 256. Heads that fill
+// those by themselves are not cut. Else n segments take about chunks / n * 9 us
+// for their two passes and n states of all heads, moved five times at 4 MB a
+// us; the sum is least at the root below.
 int attn_segments(const AttnShape& s, int type, long* seg_len) {
   const long chunks = (s.T + 63) / 64, heads = s.B * s.H;
-  const long slots = std::max(s.dk, s.dv) > 64 ? 256 : type == 0 ? 512 : 1024;
+  const long d = std::max(s.dk, s.dv);
+  const long slots = d > 64 ? 256
+                     : type == 1 || (type == 2 && d <= 32) ? 1024 : 512;
   const double best = std::sqrt(chunks * 9.0 * 4e6 /
                                 (20.0 * heads * s.dk * s.dv));
   long n = std::min({slots / heads, chunks, (long)std::min(best, 1e6)});
