@@ -531,6 +531,46 @@ def test_non_finite_gradients_stay(T, dtype):
     assert got[5].isfinite().all()
 
 
+def _same_where_finite(got, ref, mag, rel, what):
+    """Finite at the same places, and close there."""
+    ok = ref.isfinite()
+    assert torch.equal(got.isfinite().cpu(), ok), what
+    z = torch.zeros_like(ref)
+    _close(torch.where(ok.to(got.device), got, torch.zeros_like(got)),
+           torch.where(ok, ref, z), torch.where(ok, mag, z), rel, what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["q", "k", "v", "s", "do", "df"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_non_finite_crosses_segments(dtype, name, value):
+    """A decay that underflows over a segment is no done: what is not finite
+    stays so over all later segments, up to the next done."""
+    T, D = 600, 16
+    q, k, v, g, _, s, do, df = _inputs(T, 1, 2, D, D, dtype, 0)
+    g = torch.tensor([-3.0, -0.01], device="cuda")
+    d = torch.zeros(T, 1, dtype=torch.bool, device="cuda")
+    a = dict(q=q, k=k, v=v, s=s, do=do, df=df)
+    mag = _ref(q.abs(), k.abs(), v.abs(), g, d, s.abs(), 0.25, do.abs(),
+               df.abs())
+    full, rel = _bounds(dtype, T, D, D)
+    a[name] = a[name].clone()
+    if name in ("s", "df"):
+        a[name][0, 0, 5, 3] = value
+    else:
+        a[name][T - 70 if name == "do" else 70, 0, 0, 5] = value
+    for cut in (None, 130, T - 130):
+        if cut is not None:
+            d[cut] = True
+        got = _run(a["q"], a["k"], a["v"], g, d, a["s"], a["do"], a["df"])
+        ref = _ref(a["q"], a["k"], a["v"], g, d, a["s"], 0.25, a["do"],
+                   a["df"])
+        for n, x, r, m in zip(NAMES, got, ref, mag):
+            _same_where_finite(x, r, m,
+                               rel if n in ("final", "dstate") else full, n)
+
+
 @pytest.mark.gpu
 def test_nothing_to_do():
     for T, B, H in ((0, 2, 3), (4, 0, 3), (4, 2, 0)):

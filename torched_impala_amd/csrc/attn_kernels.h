@@ -31,7 +31,8 @@ struct AttnArgs {
   long g_stride;
   const unsigned char* done;   // (T, B) or null
   long done_st, done_sb;
-  float* keep;              // first pass: (nseg, B * H), a segment's decay
+  float* keep;              // first pass: (nseg, B * H), a segment's decay,
+                            //   negative where a done lies in it
   long T, seg_len;          // seg_len a multiple of 64
   int B, H, nseg;
 };

@@ -72,6 +72,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int C = 64;         // steps in a chunk: one wave's ballot of dones
+constexpr float CUT = -1.f;   // decay of a segment that a done lies in
 
 // --------------------------------------------------------------------------
 // e^{g n}: n * log2(e) * g in two floats, so that the rounding of a long
@@ -986,9 +987,10 @@ attn_chunks(AttnArgs args) {
     if (n + 1 < chunks) __syncthreads();   // LDS is free for the next chunk
   }
 
+  // a done is not a decay of zero, which many steps without one may reach
   if (STATE_ONLY && tid == 0)
     args.keep[seg * heads + bh] =
-        seen_done ? 0.f : decay.pow((float)(t_hi - t_lo));
+        seen_done ? CUT : decay.pow((float)(t_hi - t_lo));
 
   // the state behind the last step of this pass: a segment's own in the
   // first pass, the whole sequence's in the main one
@@ -1023,15 +1025,24 @@ attn_chunks(AttnArgs args) {
   }
 }
 
+// What a segment leaves of a state. A decay of a whole segment may be zero in
+// 32 bits where that of a step is not: a step then says what becomes of a state
+// that is not finite.
+__device__ inline float carry(float run, float keep, float step) {
+  if (keep == CUT) return 0.f;
+  return run * (isfinite(run) ? keep : step);
+}
+
 // own states of segments -> states that enter them, in place. first: what
 // enters the first of them (in the direction of travel), or null for zero
 __global__ void __launch_bounds__(256)
 attn_scan(float* __restrict__ st, const float* __restrict__ keep,
-          const float* __restrict__ first, long heads, long size, int nseg,
-          int rev) {
+          const float* __restrict__ first, const float* __restrict__ log_decay,
+          long g_stride, int H, long heads, long size, int nseg, int rev) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= heads * size) return;
   const long bh = i / size;
+  const float step = Decay(log_decay[bh % H * g_stride]).pow(1.f);
   float run = first ? first[i] : 0.f;
   // eight segments are read before the first is written: a load does not move
   // over a store to the same array by itself
@@ -1049,7 +1060,7 @@ attn_scan(float* __restrict__ st, const float* __restrict__ keep,
       if (n0 + e < nseg) {
         const long s = rev ? nseg - 1 - n0 - e : n0 + e;
         st[s * heads * size + i] = run;
-        run = (k[e] == 0.f ? 0.f : run * k[e]) + own[e];
+        run = carry(run, k[e], step) + own[e];
       }
     }
   }
@@ -1195,11 +1206,13 @@ void launch_attn_chunks(int type, const AttnArgs* a, int vec, int state_only,
 }
 
 void launch_attn_scan(float* st, const float* keep, const float* first,
+                      const float* log_decay, long g_stride, int H,
                       long heads, long size, int nseg, int rev,
                       hipStream_t s) {
   const long n = heads * size;
   hipLaunchKernelGGL(attn_scan, dim3((unsigned)((n + 255) / 256)), dim3(256),
-                     0, s, st, keep, first, heads, size, nseg, rev);
+                     0, s, st, keep, first, log_decay, g_stride, H, heads,
+                     size, nseg, rev);
 }
 
 void launch_attn_step(int type, const AttnStepArgs* a, int vec,

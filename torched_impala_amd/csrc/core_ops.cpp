@@ -34,8 +34,8 @@ void launch_layer_norm_bwd(int, int, int, const void*, const void*, long,
                            float*, void*, void*, long, long, hipStream_t);
 void launch_attn_chunks(int, const impala::attn::AttnArgs*, int, int,
                         hipStream_t);
-void launch_attn_scan(float*, const float*, const float*, long, long, int,
-                      int, hipStream_t);
+void launch_attn_scan(float*, const float*, const float*, const float*, long,
+                      int, long, long, int, int, hipStream_t);
 void launch_attn_step(int, const impala::attn::AttnStepArgs*, int,
                       hipStream_t);
 void launch_ns_start(impala::ortho::Args*, hipStream_t);
@@ -391,8 +391,8 @@ Tensor attn_entry_states(AttnArgs a, const AttnRole& role,
   a.role[0].s_out = st.data_ptr<float>();
   a.keep = keep.data_ptr<float>();
   launch_attn_chunks(type, &a, vec, 1, stream);
-  launch_attn_scan(st.data_ptr<float>(), a.keep, first, heads, size, a.nseg,
-                   role.rev, stream);
+  launch_attn_scan(st.data_ptr<float>(), a.keep, first, a.log_decay,
+                   a.g_stride, a.H, heads, size, a.nseg, role.rev, stream);
   return st;
 }
 
