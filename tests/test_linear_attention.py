@@ -572,6 +572,41 @@ def test_non_finite_crosses_segments(dtype, name, value):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [40, 150, 600])
+@pytest.mark.parametrize("D", [16, 48, 128])
+@pytest.mark.parametrize("e", [40, 60])
+def test_fp16_zero_columns_under_a_large_scale(T, D, e):
+    """Columns of zeros have no size to be scaled by: a scale far beyond
+    fp16's range leaves them zero.
+
+    q and do lie among fp16's subnormals, whose products the matrix
+    instruction adds at the place of 2^-14: a subnormal's exponent field is
+    that of 2^-14, and nothing moves its leading zeros out. The sums' roundings
+    are then those of magnitudes of 2^-14 or more (measured over 32 products
+    of operands of 2^-20: 2^-19.5 of their magnitudes' sum, 2^-23.6 of normal
+    ones), so the bound's magnitudes are taken so."""
+    q, k, v, g, d, s, do, df = _inputs(T, 1, 2, D, D, torch.float32, 0.01)
+    q, k, v, do = ((t * 2.0 ** x).half()
+                   for t, x in ((q, -20), (k, -10), (v, 20 - e // 2 - 10),
+                                (do, -20)))
+    do[..., ::2] = 0
+    k[..., 1::2] = 0
+    v[..., 1::3] = 0
+    s[..., 1::3] = 0
+    df[..., ::2] = 0
+    got = _run(q, k, v, g, d, s, do, df, scale=2.0 ** e)
+    ref = _ref(q, k, v, g, d, s, 2.0 ** e, do, df)
+    mag = _ref(*(torch.where(t == 0, 0, t.abs().clamp_min(2.0 ** -14))
+                 for t in (q, k, v)), g, d, s.abs(), 2.0 ** e,
+               torch.where(do == 0, 0, do.abs().clamp_min(2.0 ** -14)),
+               df.abs())
+    full, rel = _bounds(q.dtype, T, D, D)
+    for n, x, r, m in zip(NAMES, got, ref, mag):
+        _close(x, r, m, rel if n in ("final", "dstate") else full, n)
+        assert not x[(m == 0).to(x.device)].any(), n
+
+
+@pytest.mark.gpu
 def test_nothing_to_do():
     for T, B, H in ((0, 2, 3), (4, 0, 3), (4, 2, 0)):
         q, k, v, g, d, s, do, df = _inputs(T, B, H, 4, 5, torch.float32)
