@@ -607,6 +607,47 @@ def test_fp16_zero_columns_under_a_large_scale(T, D, e):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [16, 128])
+@pytest.mark.parametrize("g", [1.0, 1.395, 3.0, 80.0])
+@pytest.mark.parametrize("T", [64, 600])
+def test_growing_zeros(dtype, D, g, T):
+    """Decays above zero, whose powers overflow: zeros stay zeros."""
+    q, k, v, _, d, s, do, df = (
+        torch.zeros_like(t) for t in _inputs(T, 1, 2, D, D, dtype))
+    g = torch.tensor([g, -0.1], device="cuda")
+    for n, x in zip(NAMES, _run(q, k, v, g, d, s, do, df)):
+        assert not x.any(), n
+    for n, x in zip(NAMES, _run(q, k, v, g, None, None, do, None)):
+        assert not x.any(), n
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("g,T", [(0.02, 1500), (0.5, 150), (1.395, 63),
+                                 (1.395, 64), (3.0, 28)])
+@pytest.mark.parametrize("D", [16, 128])
+@pytest.mark.parametrize("state", [False, True])
+def test_growing_states(g, T, D, state):
+    """Results within 32 bits where a decay's powers are not. Step by step a
+    contribution is rounded twice a step and scaled by a decay that is off by
+    two more, which 4 T more roundings cover."""
+    a = _inputs(T, 1, 2, D, D, torch.float32, 0.02, state)
+    for i in (0, 1, 5, 7):   # q, k and the states
+        if a[i] is not None:
+            a[i] = a[i] * 2.0 ** -20
+    a[3] = torch.tensor([g, -0.1], device="cuda")
+    q, k, v, g, d, s, do, df = a
+    got = _run(*a, scale=0.25)
+    ref = _ref(q, k, v, g, d, s, 0.25, do, df)
+    mag = _ref(q.abs(), k.abs(), v.abs(), g, d,
+               None if s is None else s.abs(), 0.25, do.abs(),
+               None if df is None else df.abs())
+    rel = _bounds(q.dtype, T, D, D)[1] + 4 * T * U
+    for n, x, r, m in zip(NAMES, got, ref, mag):
+        _close(x, r, m, rel, n)
+
+
+@pytest.mark.gpu
 def test_nothing_to_do():
     for T, B, H in ((0, 2, 3), (4, 0, 3), (4, 2, 0)):
         q, k, v, g, d, s, do, df = _inputs(T, B, H, 4, 5, torch.float32)

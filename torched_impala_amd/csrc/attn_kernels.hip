@@ -558,6 +558,9 @@ attn_chunks(AttnArgs args) {
   }
   bool seen_done = false;
   __syncthreads();
+  // a decay above zero whose powers overflow: zeros times those are NaN, so
+  // such a head goes step by step too
+  const bool grows = !(pw[C] <= 3.4e38f);
 
   // Blocks of P on and under the diagonal: with SHARE the wave's own of the
   // ten, else the four distances from it. e^{g (i - j)} at the lane's places
@@ -818,7 +821,7 @@ attn_chunks(AttnArgs args) {
             for (int r = 0; r < 4; ++r) z[r] = fmaf(O[it][v][r], 0.f, z[r]);
           }
         }
-        finite = !__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f);
+        finite = !__any(grows || (z[0] + z[1]) + (z[2] + z[3]) != 0.f);
         if (finite) {
           const int x0 = 16 * NV * wave + 4 * g;
           if constexpr (VEC) {   // dv is a multiple of 4, 64 rows in 32 bits
@@ -931,7 +934,7 @@ attn_chunks(AttnArgs args) {
               for (int r = 0; r < 4; ++r) z[r] = fmaf(U[t][v][r], 0.f, z[r]);
             }
           }
-          finite = !__any((z[0] + z[1]) + (z[2] + z[3]) != 0.f);
+          finite = !__any(grows || (z[0] + z[1]) + (z[2] + z[3]) != 0.f);
         }
         if (finite) {
           #pragma unroll
@@ -1030,12 +1033,18 @@ attn_chunks(AttnArgs args) {
   }
 }
 
-// What a segment leaves of a state. A decay of a whole segment may be zero in
-// 32 bits where that of a step is not: a step then says what becomes of a state
-// that is not finite.
-__device__ inline float carry(float run, float keep, float step) {
+// What n steps of a segment leave of a state. The decay of them all may be zero
+// in 32 bits, or infinite, where that of a step is not: what becomes of a state
+// that is not finite is then said by a step, and of any other by all of them.
+__device__ inline float carry(float run, float keep, float step, int n) {
   if (keep == CUT) return 0.f;
-  return run * (isfinite(run) ? keep : step);
+  if (!isfinite(run)) return run * step;
+  if (isfinite(keep)) return run * keep;
+  for (int i = 0; i < n && isfinite(run); ++i) {
+    run *= step;
+    if (run == 0.f) break;
+  }
+  return run;
 }
 
 // own states of segments -> states that enter them, in place. first: what
@@ -1043,7 +1052,8 @@ __device__ inline float carry(float run, float keep, float step) {
 __global__ void __launch_bounds__(256)
 attn_scan(float* __restrict__ st, const float* __restrict__ keep,
           const float* __restrict__ first, const float* __restrict__ log_decay,
-          long g_stride, int H, long heads, long size, int nseg, int rev) {
+          long g_stride, int H, long heads, long size, int nseg, int rev,
+          long T, long seg_len) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= heads * size) return;
   const long bh = i / size;
@@ -1065,7 +1075,9 @@ attn_scan(float* __restrict__ st, const float* __restrict__ keep,
       if (n0 + e < nseg) {
         const long s = rev ? nseg - 1 - n0 - e : n0 + e;
         st[s * heads * size + i] = run;
-        run = carry(run, k[e], step) + own[e];
+        const long left = T - s * seg_len;
+        run = carry(run, k[e], step, (int)(left < seg_len ? left : seg_len)) +
+              own[e];
       }
     }
   }
@@ -1212,12 +1224,12 @@ void launch_attn_chunks(int type, const AttnArgs* a, int vec, int state_only,
 
 void launch_attn_scan(float* st, const float* keep, const float* first,
                       const float* log_decay, long g_stride, int H,
-                      long heads, long size, int nseg, int rev,
-                      hipStream_t s) {
+                      long heads, long size, int nseg, int rev, long T,
+                      long seg_len, hipStream_t s) {
   const long n = heads * size;
   hipLaunchKernelGGL(attn_scan, dim3((unsigned)((n + 255) / 256)), dim3(256),
                      0, s, st, keep, first, log_decay, g_stride, H, heads,
-                     size, nseg, rev);
+                     size, nseg, rev, T, seg_len);
 }
 
 void launch_attn_step(int type, const AttnStepArgs* a, int vec,

@@ -35,7 +35,7 @@ void launch_layer_norm_bwd(int, int, int, const void*, const void*, long,
 void launch_attn_chunks(int, const impala::attn::AttnArgs*, int, int,
                         hipStream_t);
 void launch_attn_scan(float*, const float*, const float*, const float*, long,
-                      int, long, long, int, int, hipStream_t);
+                      int, long, long, int, int, long, long, hipStream_t);
 void launch_attn_step(int, const impala::attn::AttnStepArgs*, int,
                       hipStream_t);
 void launch_ns_start(impala::ortho::Args*, hipStream_t);
@@ -392,7 +392,8 @@ Tensor attn_entry_states(AttnArgs a, const AttnRole& role,
   a.keep = keep.data_ptr<float>();
   launch_attn_chunks(type, &a, vec, 1, stream);
   launch_attn_scan(st.data_ptr<float>(), a.keep, first, a.log_decay,
-                   a.g_stride, a.H, heads, size, a.nseg, role.rev, stream);
+                   a.g_stride, a.H, heads, size, a.nseg, role.rev, a.T,
+                   a.seg_len, stream);
   return st;
 }
 
