@@ -9,6 +9,7 @@ import itertools
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from torched_impala_amd.ops.layernorm import layer_norm
 
@@ -104,6 +105,32 @@ def _check(x, w, b, dy, eps=1e-5):
 
 
 # --------------------------------------------------------------- CPU
+def test_forward_mode_on_cpu():
+    """torch's ops carry a tangent on."""
+    x, w, b, t = _case((3, 5), torch.float32, torch.float32, "wb", "cpu")
+    with fw.dual_level():
+        y = layer_norm(fw.make_dual(x, t), w, b)
+        assert fw.unpack_dual(y).tangent is not None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """The kernels have no forward-mode derivative: never a result without
+    one."""
+    x, w, b, t = _case((3, 5), torch.float32, torch.float32, "wb", "cuda")
+    for i in range(3):
+        a = [x, w, b]
+        with fw.dual_level():
+            a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+            if grad:
+                a[0] = a[0].requires_grad_()
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                layer_norm(*a)
+            y = layer_norm(*a, force_eager=True)
+            assert fw.unpack_dual(y).tangent is not None
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_cpu_path(dtype):
     _check(*_case((3, 5, 19), dtype, torch.float32, "wb", "cpu"))

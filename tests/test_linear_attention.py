@@ -15,6 +15,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from torched_impala_amd.ops.linear_attention import (
     linear_attention, linear_attention_step)
@@ -151,6 +152,49 @@ def test_cpu_step_is_one_step():
     o, r = linear_attention_step(q[0], k[0], v[0], g, buf, done=d[0],
                                  out_state=buf)
     assert r is buf and not torch.equal(buf, s)
+
+
+def _refuse_forward_mode_of_a_step(device):
+    q, k, v, g, d, s, _, _ = _inputs(1, 2, 2, 4, 5, torch.float32,
+                                     device=device)
+    for i in range(6):
+        a = [q[0], k[0], v[0], g, s.clone(), torch.empty_like(s)]
+        with fw.dual_level():
+            a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                linear_attention_step(*a[:5], done=d[0], out_state=a[5])
+
+
+def test_forward_mode_on_cpu():
+    """torch's ops carry a tangent on; a step has no derivatives at all."""
+    q, k, v, g, d, s, _, _ = _inputs(3, 2, 2, 4, 5, torch.float32,
+                                     device="cpu")
+    with fw.dual_level():
+        out, fin = linear_attention(q, k, fw.make_dual(v, v), g, done=d,
+                                    state=s)
+        assert fw.unpack_dual(out).tangent is not None
+        assert fw.unpack_dual(fin).tangent is not None
+    _refuse_forward_mode_of_a_step("cpu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """The kernels have no forward-mode derivative: never a result without
+    one."""
+    q, k, v, g, d, s, _, _ = _inputs(3, 2, 2, 4, 5, torch.float32)
+    for i in range(5):
+        a = [q, k, v, g, s]
+        with fw.dual_level():
+            a[i] = fw.make_dual(a[i], torch.ones_like(a[i]))
+            if grad:
+                a[0] = a[0].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                linear_attention(*a[:4], done=d, state=a[4])
+            out, _ = linear_attention(*a[:4], done=d, state=a[4],
+                                      force_eager=True)
+            assert fw.unpack_dual(out).tangent is not None
+    _refuse_forward_mode_of_a_step("cuda")
 
 
 def test_cpu_nothing_to_do():

@@ -16,6 +16,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from torched_impala_amd.ops.orthogonal import COEFFICIENTS, orthogonalize
 
@@ -118,6 +119,25 @@ def _refuse(device):
 
 def test_refusals_cpu():
     _refuse("cpu")
+
+
+def _refuse_forward_mode(device):
+    g = _rand(6, 8, device=device)
+    with fw.dual_level():
+        dual = fw.make_dual(g, g.clone())
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            orthogonalize([g, dual])
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            orthogonalize([g], out=[dual])
+
+
+def test_forward_mode_is_refused_cpu():
+    _refuse_forward_mode("cpu")
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused_gpu():
+    _refuse_forward_mode("cuda")
 
 
 # --------------------------------------------------------------- GPU

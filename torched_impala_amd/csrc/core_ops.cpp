@@ -81,6 +81,14 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// the kernels compute no forward-mode derivatives: a tangent is refused, not
+// dropped
+void refuse_tangents(const char* op, std::initializer_list<Tensor> ts) {
+  for (const Tensor& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), op,
+                " has no forward-mode derivative");
+}
+
 // gradients of operators that are differentiable once: a second
 // differentiation raises instead of taking them for constants
 variable_list once(variable_list grads, const char* what) {
@@ -220,6 +228,7 @@ class LayerNorm : public torch::autograd::Function<LayerNorm> {
 Tensor layer_norm(Tensor x, OptTensor weight, OptTensor bias, double eps) {
   const Tensor w = or_undefined(weight), b = or_undefined(bias);
   check_norm(x, w, b, eps);
+  refuse_tangents("layer_norm", {x, w, b});
   if (wants_grad({x, w, b}))
     return LayerNorm::apply(x, weight, bias, eps);
   return norm_fwd(x, w, b, eps, false, nullptr);
@@ -556,6 +565,7 @@ std::tuple<Tensor, Tensor> linear_attention(Tensor q, Tensor k, Tensor v,
   const AttnShape s =
       check_attn("linear_attention", q, k, v, g, done, state, 2);
   const double scale = scale_of("linear_attention", scale_, s);
+  refuse_tangents("linear_attention", {q, k, v, g, state});
   if (wants_grad({q, k, v, state})) {
     auto r = LinearAttention::apply(q, k, v, g, done_, state_, scale);
     return {r[0], r[1]};
@@ -586,6 +596,7 @@ std::tuple<Tensor, Tensor> linear_attention_step(
   const double scale = scale_of(op, scale_, s);
   TORCH_CHECK(!wants_grad({q0, k0, v0, state}), op,
               " has no gradient; use linear_attention with T = 1");
+  refuse_tangents(op, {q0, k0, v0, g, state, or_undefined(out_state_)});
   const c10::DeviceGuard guard(q0.device());
   Tensor next;
   if (out_state_.has_value()) {

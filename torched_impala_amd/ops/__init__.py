@@ -69,6 +69,12 @@ def ext_for(t: torch.Tensor):
     return _EXT_HIP or ext_hip()
 
 
+def has_tangent(tensors) -> bool:
+    """Whether one of ``tensors`` carries a forward-mode derivative."""
+    return any(torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+               for t in tensors)
+
+
 def pin_host_memory(t: torch.Tensor):
     """hipHostRegister a CPU tensor's storage (page-lock for async DMA).
 

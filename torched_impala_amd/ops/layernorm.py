@@ -58,7 +58,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     ``weight`` and ``bias`` are (cols,), fp32 or of x's type, each optional.
     Returns a contiguous tensor of x's shape and type; differentiable once
     in x, weight and bias. ``force_eager`` takes torch's ops instead of the
-    kernels. Raises TypeError or ValueError for anything else.
+    kernels, which raise RuntimeError where an input carries a forward-mode
+    derivative. Raises TypeError or ValueError for anything else.
     """
     ext = None if force_eager else ops.ext_for(x)
     if ext is not None:   # checks, saves and differentiates by itself

@@ -130,7 +130,9 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     Returns ``(out, final)``: out (T, B, H, dv) of q's type and the state
     behind the last step, fp32. Differentiable once in q, k, v and state,
-    through both results; log_decay gets no gradient. NaN and infinities
+    through both results; log_decay gets no gradient. The kernels raise
+    RuntimeError where an input carries a forward-mode derivative, which
+    torch's ops carry on. NaN and infinities
     reach the steps that the recurrence carries them to, never an earlier
     step or another episode. Raises TypeError or ValueError for anything
     else.
@@ -162,7 +164,8 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``state`` itself (in place) or memory apart from it; its environments
     may lie apart (a slice of a larger pool), an environment's heads are
     contiguous. Not differentiable: raises RuntimeError where a gradient is
-    asked for (``linear_attention`` with T = 1 has one).
+    asked for (``linear_attention`` with T = 1 has one) or an input carries a
+    forward-mode derivative.
     """
     ext = ops.ext_for(q)
     if ext is not None:
@@ -174,6 +177,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             t.requires_grad for t in (q, k, v, state)):
         raise RuntimeError("linear_attention_step has no gradient; use "
                            "linear_attention with T = 1")
+    if ops.has_tangent(t for t in (q, k, v, log_decay, state, out_state)
+                       if t is not None):
+        raise RuntimeError("linear_attention_step has no forward-mode "
+                           "derivative")
     if out_state is not None:
         if out_state.dtype is not torch.float32:
             raise TypeError("linear_attention_step: out_state must be fp32, "

@@ -45,6 +45,9 @@ def _check_out(mats, out):
         if o.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("orthogonalize writes its results in place; "
                                "they must not require grad")
+    if ops.has_tangent(out):
+        raise RuntimeError("orthogonalize writes its results in place; they "
+                           "must not carry a forward-mode derivative")
     # a result may lie on its own matrix, on nothing else
     spans = sorted((*_span(o), i) for i, o in enumerate(out) if o.numel())
     for (_, e, i), (s, _, j) in zip(spans, spans[1:]):
@@ -91,8 +94,8 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5,
     Results are new contiguous tensors, or written to ``out``: dense tensors
     of the matrices' shapes and types, each apart from the other results and
     matrices (its own it may overwrite). Not differentiable: raises
-    RuntimeError where a matrix requires grad, TypeError or ValueError for
-    anything else that does not fit.
+    RuntimeError where a matrix requires grad or carries a forward-mode
+    derivative, TypeError or ValueError for anything else that does not fit.
     """
     mats = list(mats)
     for i, g in enumerate(mats):
@@ -111,6 +114,8 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5,
         if g.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("orthogonalize has no gradient; pass the "
                                "matrices detached")
+    if ops.has_tangent(mats):
+        raise RuntimeError("orthogonalize has no forward-mode derivative")
     if not isinstance(steps, int) or steps < 1:
         raise ValueError(f"orthogonalize: steps must be an integer of one "
                          f"or more, not {steps}")
