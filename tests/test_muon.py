@@ -155,6 +155,41 @@ def test_state_dict_roundtrip():
                            .state_dict())
 
 
+def _state_of(opt):
+    return ([t.clone() for t in opt.state_arenas()], opt._steps,
+            [{k: v for k, v in g.items() if k != "params"}
+             for g in opt.param_groups])
+
+
+@pytest.mark.parametrize("make", [
+    lambda net: FlatRMSprop(net.parameters(), lr=0.5),
+    lambda net: _make(net, 40.0)])
+def test_a_state_that_does_not_fit_changes_nothing(make):
+    """States of the other optimizer, of another net and damaged ones are
+    refused by name before the first average is overwritten."""
+    torch.manual_seed(0)
+    net = MLPPolicy((4,), 2, use_lstm=True)
+    opt = make(net)
+    opt.flat_sqavg.normal_()
+    muon = isinstance(opt, FlatMuon)
+    other = MLPPolicy((5,), 2, use_lstm=True)
+    states = [make(other).state_dict(),
+              FlatRMSprop(net.parameters()).state_dict() if muon
+              else _make(net, 40.0).state_dict()]
+    opt = make(net)   # the arenas are the last optimizer's that was made
+    opt.flat_sqavg.normal_()
+    damaged = opt.state_dict()
+    last = damaged["state"][len(damaged["state"]) - 1]
+    last.pop("momentum_buffer" if muon else "square_avg")
+    for sd in states + [damaged]:
+        before = _state_of(opt)
+        with pytest.raises(ValueError):
+            opt.load_state_dict(sd)
+        after = _state_of(opt)
+        assert all(torch.equal(a, b) for a, b in zip(before[0], after[0]))
+        assert before[1:] == after[1:]
+
+
 def _train_rank(rank, world, port, q):
     """Three steps of a linear-attention policy on this rank's half of the
     batch (world 2) or on all of it (world 1)."""

@@ -141,16 +141,32 @@ class FlatRMSprop(torch.optim.Optimizer):
                    "params": list(range(len(params)))}]
         return {"state": state, "param_groups": groups}
 
-    def load_state_dict(self, sd):
-        params = self.param_groups[0]["params"]
+    def _load_entries(self, sd, wanted):
+        """wanted: (parameter, key of its entry) in the state's order. An
+        entry that is missing leaves what is there; nothing is changed before
+        every entry is known to fit."""
+        found = []
+        for i, (p, key) in enumerate(wanted):
+            ent = sd["state"].get(i, sd["state"].get(str(i)))
+            if ent is None:
+                continue
+            if key not in ent:
+                raise ValueError(f"parameter {i} has no {key} in the state: "
+                                 "another optimizer's")
+            if ent[key].numel() != p.numel():
+                raise ValueError(f"parameter {i} has {p.numel()} values, "
+                                 f"{ent[key].numel()} in the state")
+            found.append((p, ent, key))
         with torch.no_grad():
-            for i, p in enumerate(params):
-                if i in sd["state"] or str(i) in sd["state"]:
-                    ent = sd["state"].get(i, sd["state"].get(str(i)))
-                    off, n = self.slices[p]
-                    self.flat_sqavg[off:off + n].copy_(
-                        ent["square_avg"].reshape(-1).to(self.flat_sqavg.device))
-                    self._steps = int(ent.get("step", self._steps))
+            for p, ent, key in found:
+                off, n = self.slices[p]
+                self.flat_sqavg[off:off + n].copy_(
+                    ent[key].reshape(-1).to(self.flat_sqavg.device))
+                self._steps = int(ent.get("step", self._steps))
+
+    def load_state_dict(self, sd):
+        self._load_entries(sd, [(p, "square_avg") for p in
+                                self.param_groups[0]["params"]])
         for k in ("lr", "alpha", "eps"):
             if sd.get("param_groups"):
                 self.param_groups[0][k] = sd["param_groups"][0].get(
@@ -291,19 +307,11 @@ class FlatMuon(FlatRMSprop):
         for g, old in zip(self.param_groups, sd["param_groups"]):
             if len(g["params"]) != len(old["params"]):
                 raise ValueError("the state's parameters do not match")
-        i = 0
-        with torch.no_grad():
-            for k, g in enumerate(self.param_groups):
-                key = "momentum_buffer" if k else "square_avg"
-                for p in g["params"]:
-                    off, cnt = self.slices[p]
-                    ent = sd["state"].get(i, sd["state"].get(str(i)))
-                    if ent is not None:
-                        self.flat_sqavg[off:off + cnt].copy_(
-                            ent[key].reshape(-1).to(self.flat_sqavg.device))
-                        self._steps = int(ent.get("step", self._steps))
-                    i += 1
-                old = sd["param_groups"][k]
-                for a in ("lr", "alpha", "eps", "momentum", "ns_steps"):
-                    if a in g:
-                        g[a] = old.get(a, g[a])
+        self._load_entries(
+            sd, [(p, "momentum_buffer" if k else "square_avg")
+                 for k, g in enumerate(self.param_groups)
+                 for p in g["params"]])
+        for g, old in zip(self.param_groups, sd["param_groups"]):
+            for a in ("lr", "alpha", "eps", "momentum", "ns_steps"):
+                if a in g:
+                    g[a] = old.get(a, g[a])
