@@ -297,6 +297,35 @@ def _plain_fp32(g, steps=5, eps=1e-7):
     return x
 
 
+def _mean_error(got, mats, want):
+    """Mean of the logarithm of the relative errors."""
+    return sum(math.log(torch.linalg.vector_norm(y.double().cpu() - w)
+                        / torch.linalg.vector_norm(w))
+               for y, w in zip(got, want)) / len(mats)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 2000), (7, 599), (12, 635), (16, 16),
+                                   (16, 256), (32, 288), (64, 500)])
+@pytest.mark.parametrize("tall", [False, True])
+def test_few_rows_beside_a_large_matrix(shape, tall):
+    """Few rows are as exact as in fp32 beside a matrix that takes the large
+    tiles too. The bound is that of the test of few rows by themselves."""
+    gen = torch.Generator().manual_seed(shape[0] * 3001 + shape[1])
+    mats = [torch.randn(shape, generator=gen) for _ in range(64)]
+    want = [_ref(g) for g in mats]
+    big = _rand(2048, 2048)
+    turn = (lambda t: t.t().contiguous()) if tall else (lambda t: t)
+    got = []
+    for i in range(0, 64, 8):
+        res = orthogonalize([turn(g).cuda() for g in mats[i:i + 4]] + [big]
+                            + [turn(g).cuda() for g in mats[i + 4:i + 8]])
+        got += [turn(x) for x in res[:4] + res[5:]]
+    own = _mean_error(got, mats, want)
+    plain = _mean_error([_plain_fp32(g.cuda()) for g in mats], mats, want)
+    assert own <= plain + math.log(1.25), (math.exp(own), math.exp(plain))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(4, 2000), (7, 599), (12, 635), (16, 16),
                                    (64, 500)])

@@ -743,6 +743,80 @@ long plan_product(ns::Args& a, int mode, int tile, long per) {
   return part;
 }
 
+// matrices that share their launches, at most MAX_MATS, in tiles of one size
+void orthogonalize_group(const std::vector<Tensor>& src,
+                         const std::vector<Tensor>& dst,
+                         const std::vector<size_t>& take, int tile, long steps,
+                         double eps) {
+  const Tensor& like = src[take[0]];
+  const c10::DeviceGuard guard(like.device());
+  hipStream_t stream = stream_here();
+  ns::Args a{};
+  a.count = (int)take.size();
+  long parts = 0;
+  for (int i = 0; i < a.count; ++i) {
+    const Tensor &s = src[take[i]], &d = dst[take[i]];
+    ns::Mat& m = a.mat[i];
+    const bool tall = s.size(0) > s.size(1);
+    const int r = tall ? 1 : 0, c = tall ? 0 : 1;
+    m.src = s.data_ptr();
+    m.src_i = s.stride(r);
+    m.src_j = s.stride(c);
+    m.dst = d.data_ptr();
+    m.dst_i = d.stride(r);
+    m.dst_j = d.stride(c);
+    m.type = type_code(s, "matrix");
+    m.m = (int)s.size(r);
+    m.n = (int)s.size(c);
+    m.mp = (m.m + tile - 1) / tile * tile;
+    m.np = (m.n + tile - 1) / tile * tile;
+    m.ex = scale_exp(m.n);
+    m.ea = scale_exp(m.m);
+    const long wide = 2L * m.mp * m.np, square = 2L * m.mp * m.mp;
+    m.x = parts;
+    m.xt[0] = m.x + wide;
+    m.xt[1] = m.xt[0] + wide;
+    m.a = m.xt[1] + wide;
+    m.b = m.a + square;
+    parts = m.b + square;
+  }
+  int norm_blocks = 0;
+  for (int i = 0; i < a.count; ++i) {
+    ns::Mat& m = a.mat[i];
+    const long want = ((long)m.m * m.n + 8191) / 8192;
+    m.norm_blocks = (int)std::min(want, (long)ns::MAX_NORM_BLOCKS);
+    a.first_norm[i] = norm_blocks;
+    norm_blocks += m.norm_blocks;
+  }
+  a.first_norm[a.count] = norm_blocks;
+  long partial = 0, per[3];
+  for (int mode = 0; mode < 3; ++mode) {
+    per[mode] = block_steps(a, mode, tile);
+    partial = std::max(partial, plan_product(a, mode, tile, per[mode]));
+  }
+  auto work = torch::empty({parts}, like.options().dtype(torch::kFloat16));
+  auto split = torch::empty({partial},
+                            like.options().dtype(torch::kFloat32));
+  auto sums = torch::empty({norm_blocks},
+                           like.options().dtype(torch::kFloat64));
+  auto rho = torch::empty({a.count}, like.options().dtype(torch::kFloat32));
+  a.parts = (_Float16*)work.data_ptr();
+  a.partial = split.data_ptr<float>();
+  a.sums = sums.data_ptr<double>();
+  a.rho = rho.data_ptr<float>();
+  a.eps = eps;
+  launch_ns_start(&a, stream);
+  for (long k = 0; k < steps; ++k) {
+    a.round = (int)k;
+    a.last = k + 1 == steps;
+    for (int mode = 0; mode < 3; ++mode) {
+      plan_product(a, mode, tile, per[mode]);
+      launch_ns_product(mode, tile, &a, stream);
+    }
+  }
+  check_launch("orthogonalize");
+}
+
 void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
                    long steps, double eps) {
   TORCH_CHECK(src.size() == dst.size() && steps >= 1 && eps >= 0.0,
@@ -761,84 +835,34 @@ void orthogonalize(std::vector<Tensor> src, std::vector<Tensor> dst,
   }
   size_t at = 0;
   while (at < src.size()) {
-    ns::Args a{};
-    std::vector<size_t> take;
+    std::vector<size_t> all, few, more;   // up to 64 rows, and the others
     long tiles128 = 0;
-    for (; at < src.size() && take.size() < ns::MAX_MATS; ++at) {
-      if (src[at].numel() == 0) continue;
-      take.push_back(at);
-      tiles128 += ((src[at].size(0) + 127) / 128) *
-                  ((src[at].size(1) + 127) / 128);
-    }
-    if (take.empty()) break;
-    const Tensor& like = src[take[0]];
-    const c10::DeviceGuard guard(like.device());
-    hipStream_t stream = stream_here();
-    // a tile of 128 needs half the reads of 64, if there are enough of them
-    const int tile = tiles128 >= 256 ? 128 : 64;
-    a.count = (int)take.size();
-    long parts = 0;
-    for (int i = 0; i < a.count; ++i) {
-      const Tensor &s = src[take[i]], &d = dst[take[i]];
-      ns::Mat& m = a.mat[i];
-      const bool tall = s.size(0) > s.size(1);
-      const int r = tall ? 1 : 0, c = tall ? 0 : 1;
-      m.src = s.data_ptr();
-      m.src_i = s.stride(r);
-      m.src_j = s.stride(c);
-      m.dst = d.data_ptr();
-      m.dst_i = d.stride(r);
-      m.dst_j = d.stride(c);
-      m.type = type_code(s, "matrix");
-      m.m = (int)s.size(r);
-      m.n = (int)s.size(c);
-      m.mp = (m.m + tile - 1) / tile * tile;
-      m.np = (m.n + tile - 1) / tile * tile;
-      m.ex = scale_exp(m.n);
-      m.ea = scale_exp(m.m);
-      const long wide = 2L * m.mp * m.np, square = 2L * m.mp * m.mp;
-      m.x = parts;
-      m.xt[0] = m.x + wide;
-      m.xt[1] = m.xt[0] + wide;
-      m.a = m.xt[1] + wide;
-      m.b = m.a + square;
-      parts = m.b + square;
-    }
-    int norm_blocks = 0;
-    for (int i = 0; i < a.count; ++i) {
-      ns::Mat& m = a.mat[i];
-      const long want = ((long)m.m * m.n + 8191) / 8192;
-      m.norm_blocks = (int)std::min(want, (long)ns::MAX_NORM_BLOCKS);
-      a.first_norm[i] = norm_blocks;
-      norm_blocks += m.norm_blocks;
-    }
-    a.first_norm[a.count] = norm_blocks;
-    long partial = 0, per[3];
-    for (int mode = 0; mode < 3; ++mode) {
-      per[mode] = block_steps(a, mode, tile);
-      partial = std::max(partial, plan_product(a, mode, tile, per[mode]));
-    }
-    auto work = torch::empty({parts}, like.options().dtype(torch::kFloat16));
-    auto split = torch::empty({partial},
-                              like.options().dtype(torch::kFloat32));
-    auto sums = torch::empty({norm_blocks},
-                             like.options().dtype(torch::kFloat64));
-    auto rho = torch::empty({a.count}, like.options().dtype(torch::kFloat32));
-    a.parts = (_Float16*)work.data_ptr();
-    a.partial = split.data_ptr<float>();
-    a.sums = sums.data_ptr<double>();
-    a.rho = rho.data_ptr<float>();
-    a.eps = eps;
-    launch_ns_start(&a, stream);
-    for (long k = 0; k < steps; ++k) {
-      a.round = (int)k;
-      a.last = k + 1 == steps;
-      for (int mode = 0; mode < 3; ++mode) {
-        plan_product(a, mode, tile, per[mode]);
-        launch_ns_product(mode, tile, &a, stream);
+    for (; at < src.size() && all.size() < ns::MAX_MATS; ++at) {
+      const Tensor& s = src[at];
+      if (s.numel() == 0) continue;
+      all.push_back(at);
+      if (std::min(s.size(0), s.size(1)) <= 64) {
+        few.push_back(at);
+      } else {
+        more.push_back(at);
+        tiles128 += ((s.size(0) + 127) / 128) * ((s.size(1) + 127) / 128);
       }
     }
-    check_launch("orthogonalize");
+    if (all.empty()) break;
+    // A tile of 128 needs half the reads of 64, if there are enough of them.
+    // Few rows stay with tiles of 64, which are the exact ones for them
+    // (beside 2048 x 2048 in tiles of 128 and by themselves: 4 x 2000 off by
+    // 2.7e-6 and 1.5e-6, where fp32 products are by 1.8e-6; 7 x 599 by 0.90
+    // and 0.56, fp32 0.69; 64 x 500 by 2.0 and 1.2, fp32 1.65). A second set
+    // of launches costs up to 145 us (2048 x 2048 with 8 of 64 x 2048: 1076
+    // against 929); few rows by themselves are faster so too (24 of 64 x 2048:
+    // 179 against 364 padded to tiles of 128).
+    if (tiles128 < 256) {
+      orthogonalize_group(src, dst, all, 64, steps, eps);
+      continue;
+    }
+    orthogonalize_group(src, dst, more, 128, steps, eps);
+    if (!few.empty()) orthogonalize_group(src, dst, few, 64, steps, eps);
   }
 }
 

@@ -19,11 +19,12 @@
 // keep the parts in the range of fp16: X is bounded by beta_k (|G| / (|G| +
 // eps), times a each round, up to 1.25), so its entries are of the order of
 // beta_k / sqrt(n), and those of A of beta_k^2 / sqrt(m).
-// Tiles of 64 add lo lo, keep the three small terms in sums of their own and
-// add hi hi to the sum every 64 values of k: the singular values of few rows
-// are nearly the same, and errors of one sign then do not average out (7 x
-// 599: off by 2e-6 on average, fp32 products by 0.8e-6; now 0.9e-6; the cost
-// is 2 %). Large matrices are at two thirds of fp32 products' error as it is.
+// Tiles of 64, which matrices of up to 64 rows always take, add lo lo, keep
+// the three small terms in sums of their own and add hi hi to the sum every 64
+// values of k: the singular values of few rows are nearly the same, and errors
+// of one sign then do not average out (7 x 599: off by 2e-6 on average, fp32
+// products by 0.8e-6; now 0.9e-6; the cost is 2 %). More rows are at half to
+// four fifths of fp32 products' error in tiles of 128 as it is.
 //
 // Measured, a round of 2048 x 2048 and 2048 x 8192: 193 us for A, 110 for B,
 // 299 for X (0.86 PFLOP/s of fp16 products, where the library's large bf16
