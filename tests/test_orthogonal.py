@@ -84,6 +84,54 @@ def test_singular_values_near_one():
     assert float(s.max()) <= 1.21 and float(s.min()) >= 0.6
 
 
+# What the bound of the test below lets through, and what it does not: the
+# rounds with sums in 64 bits and operands in one or two fp16 parts, as the
+# kernels keep them, with mistakes that kernels could make.
+
+def _parts(x):
+    """x in two fp16 parts, its largest entry at 2^13 to 2^14."""
+    s = 2.0 ** (13 - math.floor(math.log2(float(x.abs().max()))))
+    hi = (x * s).half().double()
+    return hi / s, (x * s - hi).half().double() / s
+
+
+def _in_parts(g, mistake=None, steps=5):
+    x = g.double() / (torch.linalg.vector_norm(g.double()) + 1e-7)
+    old = torch.zeros_like(x)
+    for _ in range(steps):
+        h, l = _parts(x)
+        if mistake == "one part":
+            l = torch.zeros_like(l)
+        elif mistake == "stale low part":
+            l, old = old, l
+        left = h if mistake == "left low part dropped" else h + l
+        m = left @ (h + l).T
+        if mistake == "low parts swapped":
+            m = h @ h.T + l @ l.T
+        m = sum(_parts(m)[:1 if mistake == "one part of A" else 2])
+        b = A * torch.eye(len(m), dtype=m.dtype) + B * m + C * (m @ m)
+        x = sum(_parts(b)[:1 if mistake == "one part of B" else 2]) @ (h + l)
+    return x
+
+
+MISTAKES = ["one part", "stale low part", "left low part dropped",
+            "low parts swapped", "one part of A", "one part of B"]
+
+
+@pytest.mark.parametrize("shape", [(128, 512), (256, 1568), (640, 640)])
+def test_twice_fp32_tells_parts_from_mistakes(shape):
+    """Two parts pass the bound of test_as_exact_as_fp32 and every mistake
+    fails it."""
+    gen = torch.Generator().manual_seed(shape[1])
+    mats = [torch.randn(shape, generator=gen) for _ in range(2)]
+    want = [_ref(g) for g in mats]
+    lim = _mean_error([_plain_fp32(g) for g in mats], mats, want) + math.log(2)
+    assert _mean_error([_in_parts(g) for g in mats], mats, want) <= lim
+    for mistake in MISTAKES:
+        got = [_in_parts(g, mistake) for g in mats]
+        assert _mean_error(got, mats, want) > lim, mistake
+
+
 def _refuse(device):
     g = _rand(6, 8, device=device)
     for exc, args, kw in [
@@ -324,6 +372,38 @@ def test_few_rows_beside_a_large_matrix(shape, tall):
     own = _mean_error(got, mats, want)
     plain = _mean_error([_plain_fp32(g.cuda()) for g in mats], mats, want)
     assert own <= plain + math.log(1.25), (math.exp(own), math.exp(plain))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shapes", [
+    [(640, 640)], [(256, 1568), (1024, 263), (1024, 256)],   # tiles of 64
+    [(1024, 1024)], [(1024, 1024)] * 4,      # of 64 and of 128, k split
+    [(2048, 2048), (65, 400), (100, 1000), (128, 2000), (263, 1024),
+     (1030, 2000), (2000, 1030)]])           # of 128
+def test_as_exact_as_fp32(shapes):
+    """fp32 matrices of more rows, in both sizes of tiles, with and without a
+    split k, against the same products in fp32. An operand of 22 bits is off by
+    2^-23 of each value, independently, and so is a product of K terms by
+    2^-23 sqrt(2 / K) of its magnitudes' sum; the sums, of 32 terms at a time,
+    are off by 2^-24 sqrt(K / 32) of their own size or less. fp32 products sum
+    the K terms with errors of the same kind, so neither is far below the
+    other: twice fp32's error is allowed for the mean over four matrices. One
+    part in place of two gives 2^-12, a thousand times as much."""
+    gen = torch.Generator().manual_seed(len(shapes) * 100 + shapes[0][0])
+    lists = [[torch.randn(s, generator=gen).cuda() for s in shapes]
+             for _ in range(4)]
+    got = [orthogonalize(mats) for mats in lists]
+
+    def wide(t):
+        return t if t.shape[0] <= t.shape[1] else t.t()
+
+    for i, shape in enumerate(shapes):
+        mats = [wide(m[i]) for m in lists]
+        want = [_plain_fp32(g.double()).cpu() for g in mats]
+        own = _mean_error([wide(x[i]) for x in got], mats, want)
+        plain = _mean_error([_plain_fp32(g) for g in mats], mats, want)
+        assert own <= plain + math.log(2), (shape, math.exp(own),
+                                            math.exp(plain))
 
 
 @pytest.mark.gpu
