@@ -130,17 +130,23 @@ struct DeviceScope {
 // transport: arenas are plain shm; the learner page-locks its mapping so
 // hipMemcpyAsync drains are real async DMA).
 // ---------------------------------------------------------------------------
-// false: the driver does not page-lock this memory (some hosts refuse any
-// that already exists); copies still work, staged by the runtime
-bool host_register(torch::Tensor t) {
+// Empty, or why the driver does not page-lock this memory: some hosts refuse
+// any that already exists, as an invalid argument or as not supported. Copies
+// still work then, staged by the runtime. Every other error is raised, an
+// earlier call's that shows here too.
+std::string host_register(torch::Tensor t) {
   TORCH_CHECK(!t.is_cuda(), "host_register takes a CPU tensor");
   TORCH_CHECK(t.is_contiguous(), "must be contiguous");
   void* ptr = t.data_ptr();
   size_t bytes = t.numel() * t.element_size();
+  if (bytes == 0) return "";
   hipError_t e = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
   // the error is not left behind for the next call to report
   if (e != hipSuccess) (void)hipGetLastError();
-  return e == hipSuccess || e == hipErrorHostMemoryAlreadyRegistered;
+  if (e == hipSuccess || e == hipErrorHostMemoryAlreadyRegistered) return "";
+  TORCH_CHECK(e == hipErrorInvalidValue || e == hipErrorNotSupported,
+              "hipHostRegister failed: ", hipGetErrorString(e));
+  return hipGetErrorString(e);
 }
 
 void host_unregister(torch::Tensor t) {

@@ -79,13 +79,16 @@ def pin_host_memory(t: torch.Tensor):
     """hipHostRegister a CPU tensor's storage (page-lock for async DMA).
 
     Where the driver refuses, the tensor stays pageable: copies from and to
-    it are still ordered on their stream, only slower."""
+    it are still ordered on their stream, only slower. Any other failure
+    raises RuntimeError."""
     ext = ext_hip(required=True)
     if ext is None:
         return
-    if not ext.host_register(t):
-        log.warning("the driver refused to page-lock %d bytes; copies go "
-                    "through pageable memory", t.numel() * t.element_size())
+    refused = ext.host_register(t)
+    if refused:
+        log.warning("the driver refused to page-lock %d bytes (%s); copies go "
+                    "through pageable memory",
+                    t.numel() * t.element_size(), refused)
 
 
 def unpin_host_memory(t: torch.Tensor):
