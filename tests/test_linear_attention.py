@@ -269,6 +269,47 @@ def test_refusals_cpu():
     _refuse("cpu")
 
 
+def _states_side_by_side(device):
+    """Old and new states of a pool that holds both for every environment."""
+    B, H, dk, dv = 3, 2, 4, 5
+    n = H * dk * dv
+    q, k, v, g, d, s, _, _ = _inputs(1, B, H, dk, dv, torch.float32,
+                                     device=device)
+    ref, new = linear_attention_step(q[0], k[0], v[0], g, s, done=d[0])
+    pool = torch.randn(B, 2 * n + 3, device=device)
+    part = [pool[:, i:i + n].unflatten(1, (H, dk, dv))
+            for i in (0, 1, n - 1, n, n + 3)]
+    before = pool.clone()
+    for i, o in ((0, 3), (0, 4), (4, 0), (3, 0)):
+        pool.copy_(before)
+        part[i].copy_(s)
+        kept = pool.clone()
+        out, r = linear_attention_step(q[0], k[0], v[0], g, part[i],
+                                       done=d[0], out_state=part[o])
+        assert torch.equal(out, ref) and torch.equal(r, new)
+        part[o].copy_(kept[:, (0, 0, 0, n, n + 3)[o]:][:, :n]
+                      .unflatten(1, (H, dk, dv)))
+        assert torch.equal(pool, kept)   # and nothing else was written
+    for i, o in ((0, 1), (1, 0), (0, 2), (2, 0), (2, 3), (4, 1)):
+        # the last one: an environment's new state reaches into the next's
+        if (i, o) == (4, 1):
+            b = pool.view(-1)[n + 3:].as_strided(s.shape, s.stride())
+            a = pool.view(-1).as_strided(s.shape, (n + 1, dk * dv, dv, 1))
+        else:
+            a, b = part[i], part[o]
+        with pytest.raises(ValueError, match="without being it"):
+            linear_attention_step(q[0], k[0], v[0], g, a, out_state=b)
+
+
+def test_states_side_by_side_cpu():
+    _states_side_by_side("cpu")
+
+
+@pytest.mark.gpu
+def test_states_side_by_side_gpu():
+    _states_side_by_side("cuda")
+
+
 def _refuse_heads(device):
     """More heads than a launch has threads for."""
     from torched_impala_amd.ops.linear_attention import MAX_HEADS

@@ -578,12 +578,24 @@ bool heads_contiguous(const Tensor& t) {
   return t.numel() == 0 || t.select(0, 0).is_contiguous();
 }
 
-// first byte and the byte behind the last
-std::pair<uintptr_t, uintptr_t> span_of(const Tensor& t) {
-  long n = 0;
-  for (int i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
-  const uintptr_t p = (uintptr_t)t.data_ptr();
-  return {p, p + (n + 1) * t.element_size()};
+// bytes from the first one to behind the last, of the axes from `axis` on
+long span_of(const Tensor& t, int axis) {
+  long n = 1;
+  for (int i = axis; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+  return n * t.element_size();
+}
+
+// Two tensors of environments, neither empty, without common memory: one
+// behind the other, or an environment's parts of both side by side in records
+// of one size.
+bool apart(const Tensor& a, const Tensor& b) {
+  const uintptr_t p = (uintptr_t)a.data_ptr(), q = (uintptr_t)b.data_ptr();
+  if (p + span_of(a, 0) <= q || q + span_of(b, 0) <= p) return true;
+  const long record = a.stride(0) * a.element_size();
+  if (record <= 0 || b.stride(0) * b.element_size() != record) return false;
+  const long at = q >= p ? (long)((q - p) % record)
+                         : record - 1 - (long)((p - q - 1) % record);
+  return at >= span_of(a, 1) && at + span_of(b, 1) <= record;
 }
 
 // q, k (B, H, dk), v (B, H, dv); the states' environments may lie apart
@@ -614,13 +626,10 @@ std::tuple<Tensor, Tensor> linear_attention_step(
                              next.stride(0) >= s.H * s.dk * s.dv),
                         op, ": out_state needs an environment's heads "
                         "contiguous and environments that do not overlap");
-      if (next.data_ptr() != state.data_ptr() ||
-          next.strides() != state.strides()) {
-        const auto [a0, a1] = span_of(state);
-        const auto [b0, b1] = span_of(next);
-        TORCH_CHECK_VALUE(a1 <= b0 || b1 <= a0, op, ": out_state overlaps "
-                          "the state without being it");
-      }
+      TORCH_CHECK_VALUE((next.data_ptr() == state.data_ptr() &&
+                         next.strides() == state.strides()) ||
+                            apart(next, state),
+                        op, ": out_state overlaps the state without being it");
     }
     // autograd has to see the write: the state may be saved somewhere
     if (!next.is_inference()) next.unsafeGetTensorImpl()->bump_version();

@@ -145,10 +145,25 @@ def linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     return _eager(q, k, v, log_decay, done, state, scale)
 
 
-def _span(t: torch.Tensor):
-    """First byte of a tensor's memory and the byte behind the last."""
-    n = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (n + 1) * t.element_size()
+def _span(t: torch.Tensor, axis: int) -> int:
+    """Bytes from a tensor's first one to behind the last, of the axes from
+    ``axis`` on."""
+    n = sum((s - 1) * st for s, st in zip(t.shape[axis:], t.stride()[axis:]))
+    return (n + 1) * t.element_size()
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Two tensors of environments, neither empty, without common memory: one
+    behind the other, or an environment's parts of both side by side in
+    records of one size."""
+    p, q = a.data_ptr(), b.data_ptr()
+    if p + _span(a, 0) <= q or q + _span(b, 0) <= p:
+        return True
+    record = a.stride(0) * a.element_size()
+    if record <= 0 or b.stride(0) * b.element_size() != record:
+        return False
+    at = (q - p) % record
+    return at >= _span(a, 1) and at + _span(b, 1) <= record
 
 
 def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -202,12 +217,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                                  "environments that do not overlap")
             same = (out_state.data_ptr() == state.data_ptr()
                     and out_state.stride() == state.stride())
-            if not same:
-                a0, a1 = _span(state)
-                b0, b1 = _span(out_state)
-                if a0 < b1 and b0 < a1:
-                    raise ValueError("linear_attention_step: out_state "
-                                     "overlaps the state without being it")
+            if not (same or _apart(out_state, state)):
+                raise ValueError("linear_attention_step: out_state overlaps "
+                                 "the state without being it")
     with torch.no_grad():
         out, new = _eager(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0),
                           log_decay,
