@@ -301,6 +301,45 @@ def _states_side_by_side(device):
             linear_attention_step(q[0], k[0], v[0], g, a, out_state=b)
 
 
+def _refuse_results_on_inputs(device):
+    """The new state over memory that the step still reads."""
+    q, k, v, g, d, s, _, _ = _inputs(1, 2, 2, 4, 5, torch.float32,
+                                     device=device)
+    ref, want = linear_attention_step(q[0], k[0], v[0], g, s, done=d[0])
+    assert s.numel() == 80
+    for i in range(5):
+        a = [q[0], k[0], v[0], g, d[0]]
+        pool = torch.zeros(200, device=device)
+        where = pool[40:] if i != 4 else pool[40:].view(torch.bool)
+        n = a[i].numel()
+        where[:n] = a[i].reshape(-1)
+        a[i] = where[:n].view(a[i].shape)
+        with pytest.raises(ValueError, match="overlaps an input"):
+            linear_attention_step(*a[:4], s, done=a[4],
+                                  out_state=pool[:80].view(s.shape))
+        out, new = linear_attention_step(*a[:4], s, done=a[4],
+                                         out_state=pool[80:160].view(s.shape))
+        assert torch.equal(out, ref) and torch.equal(new, want)
+    # an environment's state and query in one record
+    pool = torch.zeros(2, 48, device=device)
+    qr, sr = pool[:, :8].unflatten(1, (2, 4)), pool[:, 8:].view(s.shape)
+    qr.copy_(q[0])
+    sr.copy_(s)
+    out, new = linear_attention_step(qr, k[0], v[0], g, sr, done=d[0],
+                                     out_state=sr)
+    assert torch.equal(out, ref) and torch.equal(new, want)
+    assert torch.equal(qr, q[0])
+
+
+def test_results_on_inputs_are_refused_cpu():
+    _refuse_results_on_inputs("cpu")
+
+
+@pytest.mark.gpu
+def test_results_on_inputs_are_refused_gpu():
+    _refuse_results_on_inputs("cuda")
+
+
 def test_states_side_by_side_cpu():
     _states_side_by_side("cpu")
 

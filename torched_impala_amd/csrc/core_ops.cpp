@@ -630,6 +630,10 @@ std::tuple<Tensor, Tensor> linear_attention_step(
                          next.strides() == state.strides()) ||
                             apart(next, state),
                         op, ": out_state overlaps the state without being it");
+      // a block reads its inputs while others write their states
+      for (const Tensor& t : {q0, k0, v0, g, done})
+        TORCH_CHECK_VALUE(!t.defined() || apart(next, t), op,
+                          ": out_state overlaps an input");
     }
     // autograd has to see the write: the state may be saved somewhere
     if (!next.is_inference()) next.unsafeGetTensorImpl()->bump_version();

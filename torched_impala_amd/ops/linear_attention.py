@@ -176,9 +176,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     (B, H, dk, dv) fp32, done (B,). Returns ``(out, new_state)``.
 
     The new state is written to ``out_state`` if given, which may be
-    ``state`` itself (in place) or memory apart from it; its environments
-    may lie apart (a slice of a larger pool), an environment's heads are
-    contiguous. Not differentiable: raises RuntimeError where a gradient is
+    ``state`` itself (in place) or memory apart from it, and is apart from all
+    other inputs; its environments may lie apart (a slice of a larger pool),
+    an environment's heads are contiguous. Not differentiable: raises RuntimeError where a gradient is
     asked for (``linear_attention`` with T = 1 has one) or an input carries a
     forward-mode derivative.
     """
@@ -220,6 +220,10 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             if not (same or _apart(out_state, state)):
                 raise ValueError("linear_attention_step: out_state overlaps "
                                  "the state without being it")
+            if not all(_apart(out_state, t) for t in (q, k, v, log_decay, done)
+                       if t is not None):
+                raise ValueError("linear_attention_step: out_state overlaps "
+                                 "an input")
     with torch.no_grad():
         out, new = _eager(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0),
                           log_decay,
