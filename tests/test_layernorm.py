@@ -215,6 +215,13 @@ def test_strides_and_alignment():
 
 
 @pytest.mark.gpu
+def test_more_columns_than_a_launch_has_threads():
+    """Of the column sums, 32 threads a column: 2^26 columns and some."""
+    _check(*_case((2, 2 ** 26 + 40), torch.float16, torch.float16, "wb",
+                  "cuda"))
+
+
+@pytest.mark.gpu
 def test_no_rows():
     x = torch.randn(0, 33, device="cuda", requires_grad=True)
     w = torch.ones(33, device="cuda", requires_grad=True)

@@ -383,17 +383,18 @@ __global__ void __launch_bounds__(512)
 ln_cols_long(const T* __restrict__ dy, const T* __restrict__ x, long xs,
              const float* __restrict__ mean, const float* __restrict__ rstd,
              float* __restrict__ part, long rows, long cols) {
-  const long c = (long)blockIdx.x * 512 + threadIdx.x;
-  if (c >= cols) return;
-  float aw = 0.f, ab = 0.f;
-  for (long r = blockIdx.y; r < rows; r += gridDim.y) {
-    const float g = (float)dy[r * cols + c];
-    aw = fmaf(g, ((float)x[r * xs + c] - mean[r]) * rstd[r], aw);
-    ab += g;
-  }
   float* dst = part + (long)blockIdx.y * 2 * cols;
-  dst[c] = aw;
-  dst[cols + c] = ab;
+  for (long c = (long)blockIdx.x * 512 + threadIdx.x; c < cols;
+       c += (long)gridDim.x * 512) {
+    float aw = 0.f, ab = 0.f;
+    for (long r = blockIdx.y; r < rows; r += gridDim.y) {
+      const float g = (float)dy[r * cols + c];
+      aw = fmaf(g, ((float)x[r * xs + c] - mean[r]) * rstd[r], aw);
+      ab += g;
+    }
+    dst[c] = aw;
+    dst[cols + c] = ab;
+  }
 }
 
 // part[blocks][2 * cols] -> dw, db. 16 columns x 32 row shares a block (64 x 8
@@ -405,29 +406,32 @@ ln_reduce(const float* __restrict__ part, int blocks, long cols,
           W* __restrict__ dw, W* __restrict__ db) {
   __shared__ float s[32][17];
   const int lane = threadIdx.x & 15, k = threadIdx.x >> 4;
-  const long c = (long)blockIdx.x * 16 + lane;
   const long n = 2 * cols;
-  float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
-  if (c < n) {
-    int i = k;
-    for (; i + 96 < blocks; i += 128) {
-      a0 += part[(long)i * n + c];
-      a1 += part[(long)(i + 32) * n + c];
-      a2 += part[(long)(i + 64) * n + c];
-      a3 += part[(long)(i + 96) * n + c];
+  for (long c0 = (long)blockIdx.x * 16; c0 < n; c0 += (long)gridDim.x * 16) {
+    const long c = c0 + lane;
+    float a0 = 0.f, a1 = 0.f, a2 = 0.f, a3 = 0.f;
+    if (c < n) {
+      int i = k;
+      for (; i + 96 < blocks; i += 128) {
+        a0 += part[(long)i * n + c];
+        a1 += part[(long)(i + 32) * n + c];
+        a2 += part[(long)(i + 64) * n + c];
+        a3 += part[(long)(i + 96) * n + c];
+      }
+      for (; i < blocks; i += 32) a0 += part[(long)i * n + c];
     }
-    for (; i < blocks; i += 32) a0 += part[(long)i * n + c];
-  }
-  s[k][lane] = (a0 + a1) + (a2 + a3);
-  __syncthreads();
-  if (k == 0 && c < n) {
-    float v = 0.f;
-    #pragma unroll
-    for (int i = 0; i < 32; ++i) v += s[i][lane];
-    if (c < cols) {
-      if (dw) dw[c] = (W)v;
-    } else {
-      if (db) db[c - cols] = (W)v;
+    __syncthreads();   // the columns before these are written
+    s[k][lane] = (a0 + a1) + (a2 + a3);
+    __syncthreads();
+    if (k == 0 && c < n) {
+      float v = 0.f;
+      #pragma unroll
+      for (int i = 0; i < 32; ++i) v += s[i][lane];
+      if (c < cols) {
+        if (dw) dw[c] = (W)v;
+      } else {
+        if (db) db[c - cols] = (W)v;
+      }
     }
   }
 }
@@ -560,6 +564,12 @@ void with_types(int xt, int wt, F&& f) {
   else f((f16_t*)nullptr, (f16_t*)nullptr);
 }
 
+// blocks of 512 threads along one axis of a launch, which has at most 2^32
+// threads; the kernels walk on behind the last block
+inline unsigned blocks_512(long n) {
+  return (unsigned)(n < (1L << 22) ? n : 1L << 22);
+}
+
 inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
@@ -630,7 +640,7 @@ void launch_layer_norm_bwd(int xt, int wt, int aligned, const void* dy,
       blocks = (int)(rows < 64 ? rows : 64);
       if (part)
         hipLaunchKernelGGL((ln_cols_long<T>),
-                           dim3((unsigned)((cols + 511) / 512), blocks),
+                           dim3(blocks_512((cols + 511) / 512), blocks),
                            dim3(512), 0, s, (const T*)dy, (const T*)x, xs,
                            mean, rstd, part, rows, cols);
     } else {
@@ -648,7 +658,7 @@ void launch_layer_norm_bwd(int xt, int wt, int aligned, const void* dy,
     }
     if (part)
       hipLaunchKernelGGL((ln_reduce<W>),
-                         dim3((unsigned)((2 * cols + 15) / 16)), dim3(512),
+                         dim3(blocks_512((2 * cols + 15) / 16)), dim3(512),
                          0, s, part, blocks, cols, (W*)dw, (W*)db);
   });
 }
