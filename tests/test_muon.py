@@ -267,6 +267,30 @@ def test_non_finite_step_is_skipped_gpu():
 
 
 @pytest.mark.gpu
+def test_equal_gradients_give_equal_weights():
+    """Ranks hold the same gradients and each computes its own update: the
+    weights must not drift apart by the order in which a norm is added."""
+    torch.manual_seed(0)
+    net = ShallowNet((4, 84, 84), 6, use_lstm=True).cuda()
+    opt = _make(net, 0.5)
+    opt.zero_grad()
+    opt.flat_grad.normal_()
+    opt.sync_lr()
+    start = [t.clone() for t in opt.state_arenas()]
+    first = None
+    for _ in range(40):
+        for t, was in zip(opt.state_arenas(), start):
+            t.copy_(was)
+        opt.step_device()
+        got = [opt.norm_sq] + opt.state_arenas()
+        if first is None:
+            first = [t.clone() for t in got]
+            want = float(opt.flat_grad.double().square().sum())
+            assert abs(float(opt.norm_sq) / want - 1) < 1e-5
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.gpu
 def test_captured_step():
     torch.manual_seed(0)
     nets = [MLPPolicy((4,), 2, use_lstm=True).cuda() for _ in range(2)]

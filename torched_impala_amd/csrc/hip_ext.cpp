@@ -40,7 +40,7 @@ void launch_lstm_seq_bwd(const float*, const float*, const float*,
                          const float*, const float*, const float*,
                          const float*, const void*, int, int, float*,
                          float*, float*, int, hipStream_t);
-void launch_grad_sqnorm(const float*, long, const float*, float*,
+void launch_grad_sqnorm(const float*, long, const float*, float*, float*,
                         hipStream_t);
 void launch_rmsprop_update(float*, const float*, float*, long, const float*,
                            const float*, const float*, float, float, float,
@@ -350,7 +350,7 @@ void fused_clip_rmsprop(torch::Tensor flat_p, torch::Tensor flat_g,
   hipStream_t stream = current_stream();
   if (max_norm > 0.0) {
     launch_grad_sqnorm(flat_g.data_ptr<float>(), n, scale.data_ptr<float>(),
-                       norm_sq.data_ptr<float>(), stream);
+                       norm_sq.data_ptr<float>(), nullptr, stream);
   }
   launch_rmsprop_update(flat_p.data_ptr<float>(), flat_g.data_ptr<float>(),
                         flat_sqavg.data_ptr<float>(), n,
@@ -361,16 +361,20 @@ void fused_clip_rmsprop(torch::Tensor flat_p, torch::Tensor flat_g,
 }
 
 // the same steps one by one, for an arena that two updates share: the norm
-// over all of it (norm_sq zeroed by the caller), then each update its part
+// over all of it, written and added in one order, then each update its part.
+// What is orthogonalised enlarges a last bit up to 485 times, and ranks that
+// hold the same gradients would drift apart by it.
 void grad_sqnorm(torch::Tensor flat_g, torch::Tensor scale,
                  torch::Tensor norm_sq) {
   check_f32(flat_g, "flat_g");
   check_f32(scale, "scale");
   check_f32(norm_sq, "norm_sq");
+  TORCH_CHECK(flat_g.numel() > 0, "no gradients");
   DeviceScope guard(flat_g.get_device());
+  auto part = torch::empty({256}, flat_g.options());
   launch_grad_sqnorm(flat_g.data_ptr<float>(), flat_g.numel(),
                      scale.data_ptr<float>(), norm_sq.data_ptr<float>(),
-                     current_stream());
+                     part.data_ptr<float>(), current_stream());
   HIP_CHECK(hipGetLastError());
 }
 

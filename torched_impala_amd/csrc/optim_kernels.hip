@@ -15,9 +15,12 @@ namespace impala {
 // block-reduced sum of squares, ONE atomic per block (a same-word fp32
 // atomic costs ~11-13 ns serialized on this chip — per-wave atomics at
 // 4k waves measured 54 us; per-block + small grid is ~50x cheaper).
+// With `part` the blocks leave their sums there instead, for an order that
+// does not change.
 __global__ void grad_sqnorm_kernel(const float* __restrict__ g, long n,
                                    const float* __restrict__ scale,
-                                   float* __restrict__ out) {
+                                   float* __restrict__ out,
+                                   float* __restrict__ part) {
   __shared__ float s_part[4];  // one partial per wave (256 threads)
   const float s = scale[0];
   float acc = 0.f;
@@ -34,8 +37,24 @@ __global__ void grad_sqnorm_kernel(const float* __restrict__ g, long n,
   if ((threadIdx.x & 63) == 0) s_part[wave] = acc;
   __syncthreads();
   if (threadIdx.x == 0) {
-    atomicAdd(out, s_part[0] + s_part[1] + s_part[2] + s_part[3]);
+    const float sum = s_part[0] + s_part[1] + s_part[2] + s_part[3];
+    if (part) part[blockIdx.x] = sum;
+    else atomicAdd(out, sum);
   }
+}
+
+// up to 256 blocks' sums, added in one order
+__global__ void __launch_bounds__(256)
+sqnorm_parts_kernel(const float* __restrict__ part, int blocks,
+                    float* __restrict__ out) {
+  __shared__ float s_part[4];
+  float acc = (int)threadIdx.x < blocks ? part[threadIdx.x] : 0.f;
+  #pragma unroll
+  for (int off = 32; off > 0; off >>= 1) acc += __shfl_down(acc, off, 64);
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    out[0] = (s_part[0] + s_part[1]) + (s_part[2] + s_part[3]);
 }
 
 // p -= lr * clip(g*scale) / (sqrt(sqavg') + eps);  sqavg' updated in place.
@@ -117,13 +136,17 @@ void launch_muon_momentum(const float* g, float* mom, float* upd, long n,
                      max_norm, mu, skip_count);
 }
 
+// part: null, and the sum is added to out; or 256 floats, and it is written
 void launch_grad_sqnorm(const float* g, long n, const float* scale,
-                        float* out, hipStream_t stream) {
+                        float* out, float* part, hipStream_t stream) {
   const int block = 256;
   long grid = (n + block - 1) / block;
   if (grid > 256) grid = 256;
   hipLaunchKernelGGL(impala::grad_sqnorm_kernel, dim3((int)grid), dim3(block),
-                     0, stream, g, n, scale, out);
+                     0, stream, g, n, scale, out, part);
+  if (part)
+    hipLaunchKernelGGL(impala::sqnorm_parts_kernel, dim3(1), dim3(256), 0,
+                       stream, part, (int)grid, out);
 }
 
 void launch_rmsprop_update(float* p, const float* g, float* sqavg, long n,
