@@ -1033,14 +1033,17 @@ attn_chunks(AttnArgs args) {
   }
 }
 
-// What n steps of a segment leave of a state. The decay of them all may be zero
-// in 32 bits, or infinite, where that of a step is not: what becomes of a state
-// that is not finite is then said by a step, and of any other by all of them.
-__device__ inline float carry(float run, float keep, float step, int n) {
+// What n steps of a segment leave of a state where it or their decay is not
+// finite. The decay of them all may be zero in 32 bits, or infinite, where that
+// of a step is not: what becomes of a state that is not finite is then said by
+// a step, and of any other by all of them.
+__device__ __attribute__((noinline)) float carry_steps(float run, float keep,
+                                                       float log_decay,
+                                                       long n) {
   if (keep == CUT) return 0.f;
+  const float step = Decay(log_decay).pow(1.f);
   if (!isfinite(run)) return run * step;
-  if (isfinite(keep)) return run * keep;
-  for (int i = 0; i < n && isfinite(run); ++i) {
+  for (long i = 0; i < n && isfinite(run); ++i) {
     run *= step;
     if (run == 0.f) break;
   }
@@ -1057,7 +1060,6 @@ attn_scan(float* __restrict__ st, const float* __restrict__ keep,
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
   if (i >= heads * size) return;
   const long bh = i / size;
-  const float step = Decay(log_decay[bh % H * g_stride]).pow(1.f);
   float run = first ? first[i] : 0.f;
   // eight segments are read before the first is written: a load does not move
   // over a store to the same array by itself
@@ -1075,9 +1077,14 @@ attn_scan(float* __restrict__ st, const float* __restrict__ keep,
       if (n0 + e < nseg) {
         const long s = rev ? nseg - 1 - n0 - e : n0 + e;
         st[s * heads * size + i] = run;
-        const long left = T - s * seg_len;
-        run = carry(run, k[e], step, (int)(left < seg_len ? left : seg_len)) +
-              own[e];
+        if (isfinite(run) && k[e] <= 3.4e38f) {
+          run *= fmaxf(k[e], 0.f);
+        } else {
+          const long left = T - s * seg_len;
+          run = carry_steps(run, k[e], log_decay[bh % H * g_stride],
+                            left < seg_len ? left : seg_len);
+        }
+        run += own[e];
       }
     }
   }
